@@ -22,8 +22,8 @@
  * Any alignment is accepted; 16-byte aligned pointers with widths that are multiples of 8
  * elements take the 128-bit fast paths, everything else a scalar path with identical results.
  * Exceptions, which have 128-bit kernels only and return cudaErrorNotSupported for a pointer that is
- * not 16-byte aligned: the causal conv, the full-attention pre-processing, and the operators fused
- * with NVFP4 quantisation.
+ * not 16-byte aligned: the causal conv, the full-attention pre-processing, the operators fused
+ * with NVFP4 quantisation, and the FP8 operators with a scale per block of 128.
  */
 #ifndef Q3X_B200_H_
 #define Q3X_B200_H_
@@ -49,6 +49,7 @@ extern "C" {
 #define Q3X_B200_GDN_HEAD_DIM 128
 #define Q3X_B200_GDN_CHANNELS 10240
 #define Q3X_B200_NVFP4_BLOCK 16
+#define Q3X_B200_FP8_BLOCK 128
 
 int q3x_b200_abi_version(void);
 /* cudaGetErrorString of a value returned by any entry point (diagnostics only). */
@@ -511,6 +512,46 @@ int q3x_b200_fp8_gemv(const uint8_t* weights, float weight_scale, const uint16_t
 int q3x_b200_nvfp4_gemv(const uint8_t* packed_weights, const uint8_t* block_scales, float weight_scale_2,
                         const uint16_t* activation, size_t rows, size_t cols, float* out_f32,
                         uint16_t* out_bf16, void* stream);
+
+/* ---------------------------------------------------------------- FP8 with a scale per block of 128
+ * No counterpart in the reference, whose FP8 weights carry one scale per tensor and multiply bf16 activations
+ * (src/kernels/reference/gemv_reference.cpp:113-140).  E4M3 codes and FP32 scales on both sides of a projection:
+ *   activations [T, K]: codes [T, K], one scale per token and block of 128 columns, stored BLOCK-MAJOR as
+ *                       scales [ceil(K / 128), T] (neighbouring tokens of one block are neighbours in memory);
+ *   weights     [N, K]: codes [N, K], one scale per 128 x 128 block, scales [ceil(N / 128), ceil(K / 128)].
+ * The last block of either dimension may be shorter.  Quantisation of y (FP32, the operator's result, NOT rounded to
+ * bf16 first): amax = largest finite |y| of the block, scale = amax == 0 ? 1 : max(amax / 448, 2^-126),
+ * code = E4M3(y * (1 / scale)) to nearest even, saturating; a NaN gives the NaN code 0x7f, an infinity +-448.
+ * Widths must be multiples of 16 (cudaErrorInvalidValue); scales are 4-byte aligned, every other pointer 16-byte
+ * (cudaErrorNotSupported).  Codes and scales must not overlap each other or any other operand. */
+
+/* Codes and scales of a bf16 tensor [rows, cols]. */
+int q3x_b200_fp8_block_quantize(const uint16_t* in, size_t rows, size_t cols, uint8_t* codes, float* scales,
+                                void* stream);
+
+/* q3x_b200_residual_add_rms_norm with the FP8 operand of the next projection made in the same pass:
+ * residual_out = bf16(left + right); y = centred RMSNorm of the ROUNDED residual; codes and scales of y;
+ * normalized_out = bf16(y), or NULL to skip it.  Aliasing as for q3x_b200_residual_add_rms_norm (normalized_out may
+ * be exactly `right`).  hidden at most 32768 (else cudaErrorNotSupported). */
+int q3x_b200_residual_add_rms_norm_fp8_block(const uint16_t* left, const uint16_t* right, const uint16_t* weight,
+                                             size_t tokens, size_t hidden, float eps, uint16_t* residual_out,
+                                             uint16_t* normalized_out, uint8_t* codes, float* scales, void* stream);
+
+/* SwiGLU with the FP8 operand of the MLP down projection: codes and scales of y = silu(gate) * up over
+ * [tokens, intermediate].  Rows of gate and up are `row_stride` elements apart (a multiple of 8, else
+ * cudaErrorNotSupported; less than `intermediate` is cudaErrorInvalidValue): row_stride = intermediate for two
+ * tensors, 2 * intermediate with up = gate + intermediate for the merged layout of q3x_b200_silu_mul_merged.
+ * gate and up may overlap each other. */
+int q3x_b200_silu_mul_fp8_block(const uint16_t* gate, const uint16_t* up, size_t row_stride, size_t tokens,
+                                size_t intermediate, uint8_t* codes, float* scales, void* stream);
+
+/* The projection of those operands, for any number of tokens from one: out[t, n] (bf16, [tokens, out_features]) =
+ * sum over blocks b of activation_scales[b, t] * weight_scales[n / 128, b] * (sum over k in b of a[t, k] * w[n, k]),
+ * sums in FP32, one rounding.  in_features must be a multiple of 16, out_features of 8 (cudaErrorInvalidValue).
+ * No workspace. */
+int q3x_b200_fp8_block_gemm_bf16(const uint8_t* weights, const float* weight_scales, const uint8_t* activations,
+                                 const float* activation_scales, size_t tokens, size_t out_features,
+                                 size_t in_features, uint16_t* out, void* stream);
 
 /* launch_softmax_reference_cuda (decode_ops.h:372-374), the FP32 row softmax of softmax_reference_cpu
  * (src/runtime/reference/decode_ops.cpp:413-443): out may be exactly in. */

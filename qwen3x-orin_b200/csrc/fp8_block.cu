@@ -1,0 +1,295 @@
+// Activations in E4M3 with one FP32 scale per row and block of 128 columns, the operand of q3x_b200_fp8_block_gemm_bf16:
+// the block quantiser of a bf16 tensor, and the residual add + centred RMSNorm and the SwiGLU that quantise their result
+// in the same pass.  No counterpart in the reference (its FP8 weights carry one scale per tensor and multiply bf16
+// activations, src/kernels/reference/gemv_reference.cpp:113-140).
+//
+//   amax  = largest finite |y| of the block        scale = amax == 0 ? 1 : max(amax / 448, 2^-126)
+//   code  = E4M3(y * (1 / scale)), round to nearest even, saturating at 448; a NaN stays a NaN, an infinity saturates
+//
+// 448 is the largest E4M3 value; the floor keeps 1 / scale finite.  y is the operator's FP32 result: it is rounded once,
+// to E4M3, and not to bf16 on the way (two roundings in a row move values next to a midpoint to the wrong side).  Scales
+// lie block-major, [ceil(columns / 128), rows]: the product reads one block's scales of neighbouring rows together.
+//
+// Every kernel is a stream that reads its operands once.  A lane owns eight neighbouring columns (one 128-bit load per
+// operand, one 64-bit store of codes), sixteen lanes own a block, so a block's amax takes four shuffles and nothing leaves
+// registers between the arithmetic and the codes.
+#include "device_utils.cuh"
+#include "host_checks.hpp"
+#include "internal.hpp"
+#include "norm_math.cuh"
+#include "pointwise_ops.cuh"
+#include "q3x_b200.h"
+
+namespace q3x {
+namespace {
+
+constexpr int kBlockCols = Q3X_B200_FP8_BLOCK;    // 128
+constexpr int kBlockLanes = kBlockCols / 8;       // 16 lanes of eight columns
+constexpr float kTopE4m3 = 448.0f;
+constexpr float kSmallestScale = 1.1754943508222875e-38f;  // 2^-126
+
+// Largest finite magnitude of eight values, 0 if there is none: fmaxf drops a NaN next to a number (hence the last
+// fmaxf with 0, for eight of them), and only a vector that holds an infinity is looked at again.
+__device__ __forceinline__ float finite_amax8(const float (&y)[8]) {
+  float t = fmaxf(fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))),
+                  fmaxf(fmaxf(fabsf(y[4]), fabsf(y[5])), fmaxf(fabsf(y[6]), fabsf(y[7]))));
+  if (t == INFINITY) {
+    t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t = fmaxf(t, fabsf(y[i]) == INFINITY ? 0.0f : fabsf(y[i]));
+  }
+  return fmaxf(t, 0.0f);
+}
+__device__ __forceinline__ float block_amax(float t) {
+#pragma unroll
+  for (int o = kBlockLanes / 2; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(kFullMask, t, o));
+  return t;
+}
+__device__ __forceinline__ float scale_of_amax(float amax) {
+  return amax == 0.0f ? 1.0f : fmaxf(__fdiv_rn(amax, kTopE4m3), kSmallestScale);
+}
+// Eight codes, column i in byte i.
+__device__ __forceinline__ uint2 encode8(const float (&y)[8], float inverse) {
+  uint16_t pair[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
+        : "=h"(pair[i])
+        : "f"(__fmul_rn(y[2 * i + 1], inverse)), "f"(__fmul_rn(y[2 * i], inverse)));
+  return make_uint2(pair[0] | (static_cast<uint32_t>(pair[1]) << 16), pair[2] | (static_cast<uint32_t>(pair[3]) << 16));
+}
+
+// ---- pointwise sources: FP32 result of eight columns -----------------------------------------------------------
+struct FromTensor {
+  static constexpr bool kTwoInputs = false;
+  static __device__ __forceinline__ void apply(const uint4& a, const uint4&, float (&y)[8]) { unpack8(a, y); }
+};
+struct FromSiluMul {  // first operand = gate, second = up
+  static constexpr bool kTwoInputs = true;
+  static __device__ __forceinline__ void apply(const uint4& a, const uint4& b, float (&y)[8]) {
+    float g[8], u[8];
+    unpack8(a, g);
+    unpack8(b, u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = SiluMul::apply(g[i], u[i]);
+  }
+};
+
+constexpr int kThreads = 256;
+
+// CTA (row, split): vectors split * 256 + thread, stepping by gridDim.y * 256, of one row.
+template <class Source>
+__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const uint16_t* __restrict__ a, const uint16_t* __restrict__ b,
+                                                                 size_t row_stride, size_t rows, int row_vectors,
+                                                                 uint8_t* __restrict__ codes, float* __restrict__ scales) {
+  release_next_kernel();
+  wait_for_prior_kernels();
+  const size_t row = blockIdx.x;
+  const uint16_t* a_row = a + row * row_stride;
+  const uint16_t* b_row = Source::kTwoInputs ? b + row * row_stride : nullptr;
+  uint8_t* code_row = codes + row * static_cast<size_t>(row_vectors) * 8;
+  const int lane = threadIdx.x & 31;
+  // (the bound is that of the warp's first lane, so that all lanes take part in the shuffles)
+  for (int first = blockIdx.y * kThreads + (threadIdx.x & ~31); first < row_vectors; first += gridDim.y * kThreads) {
+    const int v = first + lane;
+    const bool valid = v < row_vectors;
+    uint4 x = make_uint4(0, 0, 0, 0), z = make_uint4(0, 0, 0, 0);
+    if (valid) {
+      x = ld_stream(a_row + static_cast<size_t>(v) * 8);
+      if (Source::kTwoInputs) z = ld_stream(b_row + static_cast<size_t>(v) * 8);
+    }
+    float y[8];
+    Source::apply(x, z, y);
+    const float scale = scale_of_amax(block_amax(finite_amax8(y)));
+    if (valid) {
+      *reinterpret_cast<uint2*>(code_row + static_cast<size_t>(v) * 8) = encode8(y, __frcp_rn(scale));
+      if ((lane & (kBlockLanes - 1)) == 0) scales[static_cast<size_t>(v / kBlockLanes) * rows + row] = scale;
+    }
+  }
+}
+
+// One CTA per row; the row stays in registers between the sum of squares and the codes.
+template <int THREADS, int VPT>
+__global__ void __launch_bounds__(THREADS) residual_norm_fp8_kernel(const uint16_t* left, const uint16_t* right,
+                                                                    const uint16_t* __restrict__ weight, size_t rows,
+                                                                    int row_vectors, float inv_width, float eps,
+                                                                    uint16_t* residual_out, uint16_t* normalized_out,
+                                                                    bool coherent, uint8_t* __restrict__ codes,
+                                                                    float* __restrict__ scales) {
+  __shared__ float scratch[THREADS / 32];
+  release_next_kernel();
+  wait_for_prior_kernels();
+  const size_t row = blockIdx.x;
+  const size_t base = row * static_cast<size_t>(row_vectors) * 8;
+  uint4 x[VPT], r[VPT];
+#pragma unroll
+  for (int k = 0; k < VPT; ++k) {
+    const int v = threadIdx.x + k * THREADS;
+    x[k] = r[k] = make_uint4(0, 0, 0, 0);
+    if (v < row_vectors) {
+      x[k] = ld_stream(left + base + v * 8);
+      r[k] = coherent ? ld_vec(right + base + v * 8) : ld_stream(right + base + v * 8);
+    }
+  }
+  float partial = 0.0f;
+#pragma unroll
+  for (int k = 0; k < VPT; ++k) {
+    const int v = threadIdx.x + k * THREADS;
+    float l[8], rr[8];
+    unpack8(x[k], l);
+    unpack8(r[k], rr);
+    add8(l, rr);
+    x[k] = pack8(l);
+    if (v < row_vectors) st_vec(residual_out + base + v * 8, x[k]);
+    partial += sum_squares8(x[k]);
+  }
+  const float inv = inverse_rms(block_sum<THREADS / 32>(partial, scratch), inv_width, eps);
+#pragma unroll
+  for (int k = 0; k < VPT; ++k) {
+    const int v = threadIdx.x + k * THREADS;
+    const bool valid = v < row_vectors;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (valid) w = ld_weight(weight + v * 8);
+    float y[8], wf[8];
+    unpack8(x[k], y);
+    unpack8(w, wf);
+    const float2 inv2 = make_float2(inv, inv);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const float2 gamma = add2(make_float2(wf[i], wf[i + 1]), make_float2(1.0f, 1.0f));
+      const float2 n = mul2(mul2(make_float2(y[i], y[i + 1]), inv2), gamma);
+      y[i] = n.x;
+      y[i + 1] = n.y;
+    }
+    // (a lane past the row's end holds 0 * inv: not NaN unless the row's own sum is, and then fmaxf drops it)
+    const float scale = scale_of_amax(block_amax(finite_amax8(y)));
+    if (valid) {
+      if (normalized_out != nullptr) st_vec(normalized_out + base + v * 8, pack8(y));
+      *reinterpret_cast<uint2*>(codes + base + v * 8) = encode8(y, __frcp_rn(scale));
+      if ((threadIdx.x & (kBlockLanes - 1)) == 0) scales[static_cast<size_t>(v / kBlockLanes) * rows + row] = scale;
+    }
+  }
+}
+
+size_t block_count(size_t cols) { return (cols + kBlockCols - 1) / kBlockCols; }
+
+// Checks of the codes and scales of a [rows, cols] result against each other; the shape is known not to overflow.
+int check_codes(const uint8_t* codes, const float* scales, size_t rows, size_t cols, host::Span* sc, host::Span* ss) {
+  using namespace host;
+  if (codes == nullptr || scales == nullptr) return kInvalid;
+  *sc = span(codes, rows * cols);
+  *ss = span(scales, rows * block_count(cols) * sizeof(float));
+  if (wraps(*sc) || wraps(*ss) || overlap(*sc, *ss)) return kInvalid;
+  return kOk;
+}
+bool codes_aligned(const uint8_t* codes, const float* scales) {
+  return host::aligned16(codes) && (reinterpret_cast<uintptr_t>(scales) & 3u) == 0;
+}
+
+template <class Source>
+int launch_quantize_rows(const uint16_t* a, const uint16_t* b, size_t row_stride, size_t rows, size_t cols, uint8_t* codes,
+                         float* scales, void* stream) {
+  using namespace host;
+  const int row_vectors = static_cast<int>(cols / 8);
+  const size_t chunks = (static_cast<size_t>(row_vectors) + kThreads - 1) / kThreads;
+  const size_t resident = resident_grid(quantize_rows_kernel<Source>, kThreads);
+  size_t splits = rows >= resident ? 1 : (resident + rows - 1) / rows;
+  if (splits > chunks) splits = chunks;
+  clear_stale_error();
+  launch_kernel(quantize_rows_kernel<Source>, dim3(static_cast<unsigned>(rows), static_cast<unsigned>(splits)), dim3(kThreads), 0,
+                as_stream(stream), latency_bound_launch(rows * splits), a, b, row_stride, rows, row_vectors, codes, scales);
+  return launch_status();
+}
+
+template <int THREADS>
+void launch_residual_norm(int vpt, size_t rows, cudaStream_t s, const uint16_t* left, const uint16_t* right,
+                          const uint16_t* weight, int row_vectors, float inv_width, float eps, uint16_t* residual_out,
+                          uint16_t* normalized_out, bool coherent, uint8_t* codes, float* scales) {
+#define Q3X_CASE(V)                                                                                                         \
+  case V:                                                                                                                   \
+    host::launch_kernel(residual_norm_fp8_kernel<THREADS, V>, dim3(static_cast<unsigned>(rows)), dim3(THREADS), 0, s,     \
+                        host::latency_bound_launch(rows), left, right, weight, rows, row_vectors, inv_width, eps,         \
+                        residual_out, normalized_out, coherent, codes, scales);                                           \
+    break;
+  switch (vpt) {
+    Q3X_CASE(1) Q3X_CASE(2) Q3X_CASE(3) Q3X_CASE(4) Q3X_CASE(5) Q3X_CASE(6) Q3X_CASE(7) Q3X_CASE(8)
+  }
+#undef Q3X_CASE
+}
+
+constexpr size_t kWidestRow = 512 * 8 * 8;  // 512 threads of eight vectors of eight columns
+
+}  // namespace
+}  // namespace q3x
+
+using namespace q3x;
+using namespace q3x::host;
+
+extern "C" int q3x_b200_fp8_block_quantize(const uint16_t* in, size_t rows, size_t cols, uint8_t* codes, float* scales,
+                                           void* stream) {
+  if (cols % 16 != 0 || mul3_overflows(rows, cols, sizeof(uint16_t))) return kInvalid;
+  if (rows == 0 || cols == 0) return kOk;
+  if (in == nullptr) return kInvalid;
+  Span sc, ss;
+  if (check_codes(codes, scales, rows, cols, &sc, &ss) != kOk) return kInvalid;
+  const Span si = span(in, rows * cols * 2);
+  if (wraps(si) || overlap(si, sc) || overlap(si, ss)) return kInvalid;
+  if (!aligned16(in) || !codes_aligned(codes, scales) || rows > 0x7fffffffu || cols > 0x7fffffffu) return kNotSupported;
+  return launch_quantize_rows<FromTensor>(in, nullptr, cols, rows, cols, codes, scales, stream);
+}
+
+extern "C" int q3x_b200_silu_mul_fp8_block(const uint16_t* gate, const uint16_t* up, size_t row_stride, size_t tokens,
+                                           size_t intermediate, uint8_t* codes, float* scales, void* stream) {
+  if (intermediate % 16 != 0 || row_stride < intermediate || mul3_overflows(tokens, row_stride, sizeof(uint16_t))) return kInvalid;
+  if (tokens == 0 || intermediate == 0) return kOk;
+  if (gate == nullptr || up == nullptr) return kInvalid;
+  Span sc, ss;
+  if (check_codes(codes, scales, tokens, intermediate, &sc, &ss) != kOk) return kInvalid;
+  const size_t bytes = ((tokens - 1) * row_stride + intermediate) * 2;  // first to last element of either operand
+  const Span sg = span(gate, bytes), su = span(up, bytes);
+  if (wraps(sg) || wraps(su)) return kInvalid;
+  if (overlap(sg, sc) || overlap(sg, ss) || overlap(su, sc) || overlap(su, ss)) return kInvalid;
+  if (!aligned16(gate) || !aligned16(up) || row_stride % 8 != 0 || !codes_aligned(codes, scales) || tokens > 0x7fffffffu ||
+      intermediate > 0x7fffffffu)
+    return kNotSupported;
+  return launch_quantize_rows<FromSiluMul>(gate, up, row_stride, tokens, intermediate, codes, scales, stream);
+}
+
+extern "C" int q3x_b200_residual_add_rms_norm_fp8_block(const uint16_t* left, const uint16_t* right, const uint16_t* weight,
+                                                        size_t tokens, size_t hidden, float eps, uint16_t* residual_out,
+                                                        uint16_t* normalized_out, uint8_t* codes, float* scales,
+                                                        void* stream) {
+  bool done;
+  const int st = check_residual_norm(left, right, weight, tokens, hidden, eps, residual_out, normalized_out, &done);
+  if (st != kOk) return st;
+  if (hidden % 16 != 0) return kInvalid;
+  if (done) return kOk;
+  Span sc, ss;
+  if (check_codes(codes, scales, tokens, hidden, &sc, &ss) != kOk) return kInvalid;
+  const size_t bytes = tokens * hidden * 2;
+  const Span others[] = {span(left, bytes), span(right, bytes), span(weight, hidden * 2), span(residual_out, bytes),
+                         span(normalized_out, normalized_out ? bytes : 0)};
+  for (const Span& o : others)
+    if (overlap(o, sc) || overlap(o, ss)) return kInvalid;
+  if (!aligned16(left) || !aligned16(right) || !aligned16(weight) || !aligned16(residual_out) ||
+      (normalized_out != nullptr && !aligned16(normalized_out)) || !codes_aligned(codes, scales) || hidden > kWidestRow ||
+      tokens > 0x7fffffffu)
+    return kNotSupported;
+  clear_stale_error();
+  const int row_vectors = static_cast<int>(hidden / 8);
+  const int threads = row_vectors <= 1024 ? 128 : row_vectors <= 2048 ? 256 : 512;
+  const int vpt = (row_vectors + threads - 1) / threads;
+  const float inv_width = 1.0f / static_cast<float>(hidden);
+  cudaStream_t s = as_stream(stream);
+  const bool coherent = normalized_out == right;
+  if (threads == 128)
+    launch_residual_norm<128>(vpt, tokens, s, left, right, weight, row_vectors, inv_width, eps, residual_out, normalized_out,
+                              coherent, codes, scales);
+  else if (threads == 256)
+    launch_residual_norm<256>(vpt, tokens, s, left, right, weight, row_vectors, inv_width, eps, residual_out, normalized_out,
+                              coherent, codes, scales);
+  else
+    launch_residual_norm<512>(vpt, tokens, s, left, right, weight, row_vectors, inv_width, eps, residual_out, normalized_out,
+                              coherent, codes, scales);
+  return launch_status();
+}

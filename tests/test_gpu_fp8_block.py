@@ -1,0 +1,328 @@
+"""GPU tests of the FP8 operators with a scale per block of 128, through the C ABI, against their definition in 64 bits
+(tests/fp8_block_util.py): sizes around whole blocks and tiles, blocks of zeros, subnormals, NaN and infinities, strides,
+streams, captured graphs, and the operators in a row as a layer uses them."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import oracle as orc
+from tests import fixtures as fx
+from tests import fp8_block_util as f8
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def g():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from tests import gpu_util
+
+    orc.build()
+    gpu_util.capi.load()
+    return gpu_util
+
+
+def bf16_values(bits):
+    return orc.bf16_decode(np.asarray(bits)).astype(np.float32)
+
+
+def rows_with_extremes(rng, rows, cols):
+    """Normal rows, and in the first blocks what a quantiser can get wrong."""
+    x = bf16_values(fx.normal_bf16(rng, (rows, cols)))
+    special = [np.zeros(16), np.full(16, np.nan), np.full(16, np.inf), np.r_[np.full(8, -np.inf), np.full(8, 3.0)],
+               np.full(16, 1e-40), np.r_[np.full(15, 1e-38), np.nan], np.full(16, 3.3e38), np.r_[np.zeros(15), 1e-45],
+               np.r_[np.full(15, -1.0), -448.0]]
+    for i, block in enumerate(special):
+        row, at = i % rows, (i // rows) * f8.BLOCK
+        if at < cols:
+            width = min(f8.BLOCK, cols - at)
+            x[row, at:at + width] = np.tile(block, 8)[:width]
+    return orc.bf16_encode(x.astype(np.float32))
+
+
+def assert_codes(got_codes, got_scales, y, relative, what=""):
+    """Codes and scales of a result y known in float64, when the kernel's own y is within `relative` of it: a scale moves
+    by that much and its one rounding, a code by half a step more."""
+    want = f8.block_scales(y.astype(np.float32)).astype(np.float64)
+    assert np.all(np.abs(got_scales - want) <= (relative + 2.0 ** -22) * want), what
+    q = y / f8.per_column(got_scales.astype(np.float64), y.shape[1])
+    got = f8.decode(got_codes)
+    assert np.array_equal(np.isnan(got), np.isnan(y)), what
+    fine = np.isfinite(y)
+    # (2^-22: the rounding of 1 / scale and of the product; 448 (1 + relative) saturates to 448)
+    slack = f8.half_step(q[fine]) + (relative + 2.0 ** -22) * np.abs(q[fine])
+    worst = np.max(np.abs(got[fine] - q[fine]) - slack) if fine.any() else 0.0
+    assert worst <= 0, f"{what}: a code is {worst} past half a step"
+
+
+# ---------------------------------------------------------------------------------------------------- quantiser
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 16), (1, 128), (1, 144), (3, 112), (9, 272), (5, 2048), (2, 2064), (300, 640),
+                                       (1, 17408), (700, 6144)])
+def test_quantize_is_bit_exact(g, rows, cols):
+    rng = np.random.default_rng([rows, cols, 7])
+    x = rows_with_extremes(rng, rows, cols)
+    codes, scales = g.empty_like_dev((rows, cols), dtype=np.uint8), g.empty_like_dev((f8.blocks_of(cols), rows), dtype=np.float32)
+    g.capi.check("q3x_b200_fp8_block_quantize", g.Dev(x), rows, cols, codes, scales, None)
+    g.sync()
+    want, want_scales = f8.quantize(bf16_values(x))
+    assert np.array_equal(scales.get(), want_scales)
+    assert np.array_equal(f8.decode(codes.get()), want, equal_nan=True)
+    assert codes.guards_intact() and scales.guards_intact()
+
+
+# ---------------------------------------------------------------------------------------------------- residual + norm
+
+
+@pytest.mark.parametrize("rows,cols,with_normalized", [(1, 16, True), (1, 5120, False), (3, 144, True), (37, 2064, True),
+                                                       (5, 8192, False), (3, 8208, True), (2, 16384, False), (2, 32768, True),
+                                                       (260, 5120, True)])
+def test_residual_norm(g, rows, cols, with_normalized):
+    rng = np.random.default_rng([rows, cols, 11])
+    left, right = fx.normal_bf16(rng, (rows, cols)), fx.normal_bf16(rng, (rows, cols))
+    weight = orc.bf16_encode((0.2 * rng.standard_normal(cols)).astype(np.float32))
+    residual, normalized = g.empty_like_dev((rows, cols)), g.empty_like_dev((rows, cols))
+    codes, scales = g.empty_like_dev((rows, cols), dtype=np.uint8), g.empty_like_dev((f8.blocks_of(cols), rows), dtype=np.float32)
+    g.capi.check("q3x_b200_residual_add_rms_norm_fp8_block", g.Dev(left), g.Dev(right), g.Dev(weight), rows, cols, 1e-6, residual,
+                 normalized if with_normalized else None, codes, scales, None)
+    g.sync()
+    want_residual = orc.bf16_encode(bf16_values(left) + bf16_values(right))
+    g.assert_bits_equal(residual.get(), want_residual, "residual")
+    r = bf16_values(want_residual).astype(np.float64)
+    y = r / np.sqrt((r * r).mean(axis=1, keepdims=True) + np.float64(np.float32(1e-6))) * (1.0 + bf16_values(weight).astype(np.float64))
+    # the FP32 y: at most 64 squares in a row and ten levels of a tree (half their error through the root), the
+    # reciprocal root's 2^-22, and three roundings -- below 2^-18
+    assert_codes(codes.get(), scales.get(), y, 2.0 ** -18, f"{rows} x {cols}")
+    if with_normalized:
+        # half a bf16 step and the FP32 error
+        got = bf16_values(normalized.get()).astype(np.float64)
+        assert np.all(np.abs(got - y) <= (2.0 ** -8 + 2.0 ** -18) * np.abs(y))
+    for d in (residual, normalized, codes, scales):
+        assert d.guards_intact()
+
+
+def test_residual_norm_in_place_of_right_and_odd_rows(g):
+    """normalized_out may be exactly `right`; a row with a NaN and one of zeros stay their own affair."""
+    rng = np.random.default_rng(13)
+    rows, cols = 4, 640
+    left, right = fx.normal_bf16(rng, (rows, cols)), fx.normal_bf16(rng, (rows, cols))
+    left[1, 5] = 0x7FC0
+    left[2], right[2] = 0, 0
+    left[3, 130] = 0x7F80
+    weight = fx.normal_bf16(rng, (cols,))
+    d_right = g.Dev(right)
+    residual, apart = g.empty_like_dev((rows, cols)), g.empty_like_dev((rows, cols))
+    blocks = f8.blocks_of(cols)
+    out = [(g.empty_like_dev((rows, cols), dtype=np.uint8), g.empty_like_dev((blocks, rows), dtype=np.float32)) for _ in range(2)]
+    args = (weight_d := g.Dev(weight), rows, cols, 1e-6, residual)
+    g.capi.check("q3x_b200_residual_add_rms_norm_fp8_block", g.Dev(left), d_right, *args, apart, *out[0], None)
+    g.capi.check("q3x_b200_residual_add_rms_norm_fp8_block", g.Dev(left), d_right, *args, d_right, *out[1], None)
+    g.sync()
+    assert weight_d is not None
+    g.assert_bits_equal(d_right.get(), apart.get(), "normalized in place")
+    for a, b in zip(out[0], out[1]):
+        assert np.array_equal(a.get(), b.get())
+    values, scales = f8.decode(out[0][0].get()), out[0][1].get()
+    assert np.isnan(values[1]).all() and np.all(scales[:, 1] == 1.0)
+    assert np.all(values[2] == 0) and np.all(scales[:, 2] == 1.0)
+    # an infinite sum normalises by 0: the finite elements vanish, the infinite one is NaN
+    assert np.isnan(values[3, 130]) and np.all(np.delete(values[3], 130) == 0)
+    # the other row is what it is alone
+    alone = g.empty_like_dev((1, cols), dtype=np.uint8), g.empty_like_dev((blocks, 1), dtype=np.float32)
+    g.capi.check("q3x_b200_residual_add_rms_norm_fp8_block", g.Dev(left[:1]), g.Dev(right[:1]), g.Dev(weight), 1, cols, 1e-6,
+                 g.empty_like_dev((1, cols)), None, *alone, None)
+    g.sync()
+    assert np.array_equal(alone[0].get()[0], out[0][0].get()[0]) and np.array_equal(alone[1].get()[:, 0], scales[:, 0])
+
+
+# ---------------------------------------------------------------------------------------------------- SwiGLU
+
+
+@pytest.mark.parametrize("rows,cols,merged", [(1, 16, False), (1, 17408, True), (7, 144, True), (33, 2064, False), (300, 1280, True),
+                                              (513, 640, False)])
+def test_silu_mul(g, rows, cols, merged):
+    rng = np.random.default_rng([rows, cols, 17])
+    both = orc.bf16_encode((3.0 * rng.standard_normal((rows, 2 * cols))).astype(np.float32))
+    both[0, 0], both[0, 1] = 0xC2C8, 0x42C8  # gates of -100 and 100
+    gate, up = both[:, :cols], both[:, cols:]
+    codes, scales = g.empty_like_dev((rows, cols), dtype=np.uint8), g.empty_like_dev((f8.blocks_of(cols), rows), dtype=np.float32)
+    if merged:
+        d = g.Dev(both)
+        g.capi.check("q3x_b200_silu_mul_fp8_block", d, d.ptr_at(cols), 2 * cols, rows, cols, codes, scales, None)
+    else:
+        g.capi.check("q3x_b200_silu_mul_fp8_block", g.Dev(gate), g.Dev(up), cols, rows, cols, codes, scales, None)
+    g.sync()
+    gv, uv = bf16_values(gate).astype(np.float64), bf16_values(up).astype(np.float64)
+    y = gv / (1.0 + np.exp(-gv)) * uv
+    # silu's FP32 error is bounded by 1e-5 (tests/test_gpu_chain_oracle.py); the product rounds once more
+    assert_codes(codes.get(), scales.get(), y, 1.1e-5, f"{rows} x {cols}")
+    assert codes.guards_intact() and scales.guards_intact()
+
+
+def test_silu_mul_non_finite(g):
+    rng = np.random.default_rng(19)
+    gate, up = fx.normal_bf16(rng, (2, 256)), fx.normal_bf16(rng, (2, 256))
+    gate[0, 3], up[1, 200], gate[1, 7], up[1, 7] = 0x7FC0, 0x7F80, 0x3F80, 0xFF80
+    codes, scales = g.empty_like_dev((2, 256), dtype=np.uint8), g.empty_like_dev((2, 2), dtype=np.float32)
+    g.capi.check("q3x_b200_silu_mul_fp8_block", g.Dev(gate), g.Dev(up), 256, 2, 256, codes, scales, None)
+    g.sync()
+    gv, uv = bf16_values(gate).astype(np.float64), bf16_values(up).astype(np.float64)
+    y = gv / (1.0 + np.exp(-gv)) * uv
+    assert_codes(codes.get(), scales.get(), y, 1.1e-5)
+    values = f8.decode(codes.get())
+    assert np.array_equal(values[np.isinf(y)], np.sign(y[np.isinf(y)]) * 448.0)
+
+
+# ---------------------------------------------------------------------------------------------------- product
+
+SHAPES = [(1, 8, 16), (1, 128, 128), (1, 5120, 5120), (2, 256, 1024), (3, 136, 2064), (16, 264, 144), (17, 128, 272), (31, 5120, 640),
+          (33, 1000, 400), (48, 640, 17408), (64, 1024, 5120), (65, 384, 1296), (100, 24, 2048), (127, 520, 640), (128, 5120, 5120),
+          (129, 256, 384), (255, 776, 1040), (256, 2048, 512), (300, 640, 6144), (512, 1288, 5120), (513, 136, 2064), (1000, 4104, 528),
+          (2049, 1032, 656)]
+
+
+def run_gemm(g, a, sa, w, sw, stream=None):
+    tokens, (n, k) = a.shape[0], w.shape
+    out = g.empty_like_dev((tokens, n), fill=0x7FC1)
+    held = [g.Dev(w), g.Dev(sw), g.Dev(a), g.Dev(sa)]
+    g.capi.check("q3x_b200_fp8_block_gemm_bf16", *held, tokens, n, k, out, stream)
+    g.sync()
+    assert out.guards_intact()
+    return out.get()
+
+
+@pytest.mark.parametrize("tokens,n,k", SHAPES)
+def test_gemm(g, tokens, n, k):
+    rng = np.random.default_rng([tokens, n, k, 23])
+    a, sa, w, sw = f8.operands(rng, tokens, n, k)
+    got = bf16_values(run_gemm(g, a, sa, w, sw)).astype(np.float64)
+    want, magnitude = f8.product(a, sa, w, sw)
+    over = np.abs(got - want) - f8.product_tolerance(want, magnitude, k)
+    assert np.max(over) <= 0, f"{np.max(over)} past the tolerance at {np.unravel_index(np.argmax(over), over.shape)}"
+
+
+@pytest.mark.parametrize("tokens,n,k", [(1, 136, 272), (16, 256, 1040), (40, 264, 640), (130, 392, 528), (600, 520, 400)])
+def test_gemm_keeps_non_finite_values_to_their_rows_and_columns(g, tokens, n, k):
+    """A NaN code, an infinite scale and scales of zero touch the outputs they belong to and no others."""
+    rng = np.random.default_rng([tokens, n, k, 29])
+    a, sa, w, sw = f8.operands(rng, tokens, n, k)
+    a[(a & 0x7F) < 0x10] |= 0x30  # no zeros or subnormals: an infinite scale gives infinities and NaN alike everywhere
+    w[(w & 0x7F) < 0x10] |= 0x30
+    clean = run_gemm(g, a, sa, w, sw)
+    row, col = tokens // 2, n // 2 + 3
+    a2, w2, sa2 = a.copy(), w.copy(), sa.copy()
+    a2[row, k - 1] = 0x7F
+    w2[col, 0] = 0xFF
+    sa2[:, tokens - 1] = 0.0
+    if tokens > 2:
+        sa2[0, 0] = np.inf
+    got = run_gemm(g, a2, sa2, w2, sw)
+    values = bf16_values(got)
+    bad = np.zeros((tokens, n), dtype=bool)
+    bad[row, :], bad[:, col] = True, True
+    assert np.isnan(values[row]).all() and np.isnan(values[:, col]).all()
+    if tokens > 2:
+        assert not np.isfinite(values[0]).any()
+        bad[0, :] = True
+    if tokens - 1 != row:
+        assert np.all(values[tokens - 1][~bad[tokens - 1]] == 0)
+        bad[tokens - 1, :] = True
+    assert np.array_equal(got[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 16, 40, 129, 700])
+def test_gemm_repeats_bit_for_bit(g, tokens):
+    """Sums are joined in one order, whatever the launch: equal inputs give equal bytes."""
+    rng = np.random.default_rng([tokens, 31])
+    a, sa, w, sw = f8.operands(rng, tokens, 520, 5136)
+    first = run_gemm(g, a, sa, w, sw)
+    for _ in range(3):
+        assert np.array_equal(run_gemm(g, a, sa, w, sw), first)
+
+
+@pytest.mark.parametrize("tokens", [1, 24, 100, 300])
+def test_gemm_on_streams_and_in_graphs(g, tokens):
+    """Two calls at once on two streams, and a captured pair replayed on new inputs."""
+    rng = np.random.default_rng([tokens, 37])
+    n, k = 1032, 2576
+    sets = [f8.operands(rng, tokens, n, k) for _ in range(2)]
+    want = [run_gemm(g, *s) for s in sets]
+    held = [[g.Dev(s[2]), g.Dev(s[3]), g.Dev(s[0]), g.Dev(s[1])] for s in sets]
+    outs = [g.empty_like_dev((tokens, n)) for _ in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    g.sync()
+    for _ in range(5):
+        for h, o, s in zip(held, outs, streams):
+            g.capi.check("q3x_b200_fp8_block_gemm_bf16", *h, tokens, n, k, o, s.cuda_stream)
+    g.sync()
+    for o, w in zip(outs, want):
+        assert np.array_equal(o.get(), w)
+    graph = torch.cuda.CUDAGraph()
+    for o in outs:
+        o.t.zero_()
+    with torch.cuda.graph(graph):
+        s = torch.cuda.current_stream().cuda_stream
+        for h, o in zip(held, outs):
+            g.capi.check("q3x_b200_fp8_block_gemm_bf16", *h, tokens, n, k, o, s)
+    graph.replay()
+    g.sync()
+    for o, w in zip(outs, want):
+        assert np.array_equal(o.get(), w)
+    for i in range(4):  # the first call's operands become the second's
+        held[0][i].t.copy_(held[1][i].t)
+    graph.replay()
+    g.sync()
+    assert np.array_equal(outs[0].get(), want[1]) and np.array_equal(outs[1].get(), want[1])
+
+
+# ---------------------------------------------------------------------------------------------------- in a row
+
+
+@pytest.mark.parametrize("tokens", [1, 19, 200])
+def test_mlp_block_in_a_row(g, tokens):
+    """Residual + norm -> merged gate | up product -> SwiGLU -> down product, captured and replayed, each stage against
+    its definition on the previous stage's own bytes."""
+    rng = np.random.default_rng([tokens, 41])
+    hidden, inter, eps = 640, 1296, 1e-6
+    left, right = fx.normal_bf16(rng, (tokens, hidden)), fx.normal_bf16(rng, (tokens, hidden))
+    weight = orc.bf16_encode((0.1 * rng.standard_normal(hidden)).astype(np.float32))
+    w1, w2 = f8.random_codes(rng, (2 * inter, hidden)), f8.random_codes(rng, (hidden, inter))
+    s1 = np.exp2(rng.uniform(-13, -11, size=(f8.blocks_of(2 * inter), f8.blocks_of(hidden)))).astype(np.float32)
+    s2 = np.exp2(rng.uniform(-13, -11, size=(f8.blocks_of(hidden), f8.blocks_of(inter)))).astype(np.float32)
+    d = {n: g.Dev(v) for n, v in dict(left=left, right=right, weight=weight, w1=w1, s1=s1, w2=w2, s2=s2).items()}
+    residual, merged, down = g.empty_like_dev((tokens, hidden)), g.empty_like_dev((tokens, 2 * inter)), g.empty_like_dev((tokens, hidden))
+    x_codes, x_scales = g.empty_like_dev((tokens, hidden), dtype=np.uint8), g.empty_like_dev((f8.blocks_of(hidden), tokens), dtype=np.float32)
+    h_codes, h_scales = g.empty_like_dev((tokens, inter), dtype=np.uint8), g.empty_like_dev((f8.blocks_of(inter), tokens), dtype=np.float32)
+
+    def enqueue(s):
+        g.capi.check("q3x_b200_residual_add_rms_norm_fp8_block", d["left"], d["right"], d["weight"], tokens, hidden, eps, residual, None,
+                     x_codes, x_scales, s)
+        g.capi.check("q3x_b200_fp8_block_gemm_bf16", d["w1"], d["s1"], x_codes, x_scales, tokens, 2 * inter, hidden, merged, s)
+        g.capi.check("q3x_b200_silu_mul_fp8_block", merged, merged.ptr_at(inter), 2 * inter, tokens, inter, h_codes, h_scales, s)
+        g.capi.check("q3x_b200_fp8_block_gemm_bf16", d["w2"], d["s2"], h_codes, h_scales, tokens, hidden, inter, down, s)
+
+    enqueue(None)
+    g.sync()
+    eager = [b.get() for b in (residual, x_codes, x_scales, merged, h_codes, h_scales, down)]
+    r = bf16_values(residual.get()).astype(np.float64)
+    y = r / np.sqrt((r * r).mean(axis=1, keepdims=True) + np.float64(np.float32(eps))) * (1.0 + bf16_values(weight).astype(np.float64))
+    assert_codes(x_codes.get(), x_scales.get(), y, 2.0 ** -18, "norm")
+    want, mag = f8.product(x_codes.get(), x_scales.get(), w1, s1)
+    assert np.all(np.abs(bf16_values(merged.get()) - want) <= f8.product_tolerance(want, mag, hidden))
+    m = bf16_values(merged.get()).astype(np.float64)
+    h = m[:, :inter] / (1.0 + np.exp(-m[:, :inter])) * m[:, inter:]
+    assert_codes(h_codes.get(), h_scales.get(), h, 1.1e-5, "SwiGLU")
+    want, mag = f8.product(h_codes.get(), h_scales.get(), w2, s2)
+    assert np.all(np.abs(bf16_values(down.get()) - want) <= f8.product_tolerance(want, mag, inter))
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        enqueue(torch.cuda.current_stream().cuda_stream)
+    for b in (residual, x_codes, x_scales, merged, h_codes, h_scales, down):
+        b.t.zero_()
+    graph.replay()
+    g.sync()
+    for b, e in zip((residual, x_codes, x_scales, merged, h_codes, h_scales, down), eager):
+        assert np.array_equal(b.get(), e) and b.guards_intact()

@@ -90,6 +90,7 @@ SIGNATURES = {
     "q3x_b200_residual_add_rms_norm_fp8_block": (_i, [_p, _p, _p, _z, _z, _f, _p, _p, _p, _p, _p]),
     "q3x_b200_silu_mul_fp8_block": (_i, [_p, _p, _z, _z, _z, _p, _p, _p]),
     "q3x_b200_fp8_block_gemm_bf16": (_i, [_p, _p, _p, _p, _z, _z, _z, _p, _p]),
+    "q3x_b200_fp8_block_gemm_error": (_i, []),
     "q3x_b200_softmax": (_i, [_p, _z, _z, _p, _p]),
     "q3x_b200_bf16_greedy_argmax": (_i, [_p, _z, _p, _p]),
 }

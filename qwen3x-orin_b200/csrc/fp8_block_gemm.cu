@@ -1,79 +1,557 @@
 // The projection of E4M3 activations with E4M3 weights, both with one FP32 scale per block of 128:
 //   out[t, n] = bf16( sum over blocks b of sa[b, t] * sw[n / 128, b] * (sum over k in b of a[t, k] * w[n, k]) )
 // sa [ceil(K / 128), T] as the quantisers of fp8_block.cu write it, sw [ceil(N / 128), ceil(K / 128)].  A block's products
-// are summed in FP32, multiplied by the two scales and added to the running FP32 sum; the one rounding is to bf16.
+// are summed in FP32 by the tensor cores, multiplied by the two scales and added to the running FP32 sum; the one rounding
+// is to bf16.
+//
+// Two kernels on tcgen05 (kind::f8f6f4: E4M3 x E4M3 -> FP32 in tensor memory), operands fetched by bulk tensor copies
+// into rings of 128-byte-swizzled stages, one stage per block of 128 columns of K:
+//   * panel: 128 tokens are the MMA's rows, 256 (or 128) outputs its columns; bound by the tensor cores;
+//   * strip: 128 outputs are the rows, 16 to 128 tokens the columns; bound by reading the weights.
+// The hardware's accumulator cannot be scaled between two blocks of K, so every block starts a fresh accumulator and the
+// scaled sum lives in registers: two accumulators alternate, and while the tensor cores fill one, the epilogue warps read
+// the other and add it, times its scale, to their FP32 sums.
+//
+// Waits are bounded; one that runs out raises a sticky word (q3x_b200_fp8_block_gemm_error), and the CTA drains its
+// copies, frees its tensor memory and returns.
+#include <cuda.h>
+
 #include "device_utils.cuh"
 #include "host_checks.hpp"
 #include "q3x_b200.h"
+#include "tcgen05.cuh"
 
 namespace q3x {
 namespace {
 
-constexpr int kBlockK = Q3X_B200_FP8_BLOCK;  // 128
-constexpr int kTile = 64, kStep = 32, kThreads = 256;
+using namespace tcgen05;
 
-__device__ __forceinline__ float2 decode2(uint32_t pair) {  // two E4M3 codes -> two floats, exactly
-  uint32_t half2;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(half2) : "h"(static_cast<uint16_t>(pair)));
-  float2 f;
-  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %2;\ncvt.f32.f16 %0, lo;\ncvt.f32.f16 %1, hi;\n}" : "=f"(f.x), "=f"(f.y) : "r"(half2));
-  return f;
+constexpr int kBlockK = Q3X_B200_FP8_BLOCK;  // 128 codes = one swizzled row of 128 bytes
+constexpr int kRowBytes = kBlockK;
+
+__device__ unsigned int g_error;
+
+// One block's product: D[128, n] = A[128, 128] B[n, 128]^T, four instructions of 32 columns of K.
+__device__ __forceinline__ void block_product(uint32_t accumulator, uint32_t a, uint32_t b, uint32_t idesc) {
+#pragma unroll
+  for (int step = 0; step < kBlockK / 32; ++step)
+    mma_e4m3(accumulator, operand_descriptor(a + step * 32), operand_descriptor(b + step * 32), idesc, step > 0 ? 1u : 0u);
 }
 
-// 64 tokens x 64 outputs per CTA, 4 x 4 per thread, codes widened to FP32 in shared memory 32 columns at a time.
-__global__ void __launch_bounds__(kThreads) block_gemm_kernel(const uint8_t* __restrict__ w, const float* __restrict__ sw,
-                                                              const uint8_t* __restrict__ a, const float* __restrict__ sa,
-                                                              size_t tokens, size_t n, size_t k, uint16_t* __restrict__ out) {
-  __shared__ float as[kStep][kTile + 4], ws[kStep][kTile + 4];
-  const size_t t0 = static_cast<size_t>(blockIdx.y) * kTile, n0 = static_cast<size_t>(blockIdx.x) * kTile;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const size_t blocks = (k + kBlockK - 1) / kBlockK;
-  float total[4][4] = {};
-  for (size_t b = 0; b < blocks; ++b) {
-    float part[4][4] = {};
-    for (int step = 0; step < kBlockK; step += kStep) {
-      const int r = threadIdx.x / 4, c = (threadIdx.x % 4) * 8;
-      const size_t col = b * kBlockK + step + c;
-      const uint2 av = t0 + r < tokens && col < k ? *reinterpret_cast<const uint2*>(a + (t0 + r) * k + col) : make_uint2(0, 0);
-      const uint2 wv = n0 + r < n && col < k ? *reinterpret_cast<const uint2*>(w + (n0 + r) * k + col) : make_uint2(0, 0);
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 fa = decode2((i < 2 ? av.x : av.y) >> (16 * (i & 1)) & 0xffffu);
-        const float2 fw = decode2((i < 2 ? wv.x : wv.y) >> (16 * (i & 1)) & 0xffffu);
-        as[c + 2 * i][r] = fa.x;
-        as[c + 2 * i + 1][r] = fa.y;
-        ws[c + 2 * i][r] = fw.x;
-        ws[c + 2 * i + 1][r] = fw.y;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int kk = 0; kk < kStep; ++kk)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) part[i][j] = fmaf(as[kk][ty * 4 + i], ws[kk][tx * 4 + j], part[i][j]);
+// (volatile, unlike a read-only load: it must stay behind wait_for_prior_kernels())
+__device__ __forceinline__ float load_scale(const float* p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+// ------------------------------------------------------------------------------------------------------------- panel
+namespace panel {
+
+constexpr int kRows = 128;                  // tokens of a tile
+constexpr int kThreads = 384;               // warp 0 fetches, warp 1 issues, warp 2 owns the tensor memory, 4 to 11 add up
+constexpr int kAdders = 8;                  // warps: 4 lane quarters x 2 column halves
+constexpr int kLaunchRegisters = 168;       // 65536 / 384, rounded down to 8
+constexpr int kBand = 16;                   // token tiles walked together
+
+template <int COLS>
+struct Shape {
+  static constexpr int kStageBytes = (kRows + COLS) * kRowBytes;
+  static constexpr int kStages = COLS == 256 ? 4 : 6;
+  static constexpr int kStoreBytes = kAdders * 32 * 128;  // a warp's 32 rows x 64 outputs
+  static constexpr int kBarriers = kStages * kStageBytes + kStoreBytes;
+  static constexpr int kShared = 1024 + kBarriers + 256;  // (1024: the stages start on a 1024-byte boundary)
+};
+
+template <int COLS>
+__global__ void __launch_bounds__(kThreads, 1)
+    block_gemm_panel_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+                            const __grid_constant__ CUtensorMap map_out, const float* __restrict__ sa,
+                            const float* __restrict__ sw, int tokens, int out_features, int blocks, int row_tiles,
+                            int col_tiles) {
+  using S = Shape<COLS>;
+  constexpr int kStages = S::kStages;
+  extern __shared__ uint8_t raw[];
+  uint8_t* shared = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const uint32_t base = shared_address(shared);
+  const uint32_t full = base + S::kBarriers, empty = full + 8 * kStages, filled = empty + 8 * kStages, drained = filled + 16;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(shared + S::kBarriers + 16 * kStages + 32);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles = row_tiles * col_tiles;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      barrier_init(full + 8 * s, 1);
+      barrier_init(empty + 8 * s, 1);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const size_t t = t0 + ty * 4 + i;
-      const float s = t < tokens ? sa[b * tokens + t] : 0.0f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const size_t o = n0 + tx * 4 + j;
-        if (o < n) total[i][j] = fmaf(__fmul_rn(s, sw[o / kBlockK * blocks + b]), part[i][j], total[i][j]);
+    for (int i = 0; i < 2; ++i) {
+      barrier_init(filled + 8 * i, 1);
+      barrier_init(drained + 8 * i, kAdders);
+    }
+    barrier_init_fence();
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(const_cast<uint32_t*>(tmem_slot))),
+                 "r"(2 * COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  // only now: a successor that took this SM's tensor memory first would wait for this kernel and this kernel for it
+  release_next_kernel();
+  wait_for_prior_kernels();
+
+  // tile -> (token tile, output tile): bands of kBand token tiles, output tiles one after the other within a band, so that
+  // the tiles in flight share their operands in L2
+  auto tile_at = [&](int tile, int& row_tile, int& col_tile) {
+    const int band = tile / (kBand * col_tiles), first = band * kBand;
+    const int height = min(kBand, row_tiles - first), rest = tile - first * col_tiles;
+    col_tile = rest / height;
+    row_tile = first + rest % height;
+  };
+
+  bool healthy = true;
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0 && lane == 0) {
+      int step = 0;
+      for (int tile = blockIdx.x; tile < tiles && healthy; tile += gridDim.x) {
+        int row_tile, col_tile;
+        tile_at(tile, row_tile, col_tile);
+        for (int b = 0; b < blocks; ++b, ++step) {
+          const int s = step % kStages;
+          if (step >= kStages && !(healthy = wait_bounded(empty + 8 * s, (step / kStages - 1) & 1))) break;
+          const uint32_t at = base + s * S::kStageBytes;
+          barrier_expect(full + 8 * s, S::kStageBytes);
+          load_box(at, &map_a, b * kBlockK, row_tile * kRows, full + 8 * s);
+          load_box(at + kRows * kRowBytes, &map_w, b * kBlockK, col_tile * COLS, full + 8 * s);
+        }
       }
+      // no copy is in flight when the CTA ends, whatever became of its readers
+      for (int last = max(0, step - kStages); last < step; ++last)
+        if (!wait_bounded(full + 8 * (last % kStages), (last / kStages) & 1)) healthy = false;
+    } else if (warp == 1 && lane == 0) {
+      int step = 0;
+      for (int tile = blockIdx.x; tile < tiles && healthy; tile += gridDim.x) {
+        for (int b = 0; b < blocks; ++b, ++step) {
+          const int s = step % kStages, half = step & 1;
+          if (step >= 2 && !(healthy = wait_bounded(drained + 8 * half, (step / 2 - 1) & 1))) break;
+          if (!(healthy = wait_bounded(full + 8 * s, (step / kStages) & 1))) break;
+          fence_after_sync();
+          const uint32_t at = base + s * S::kStageBytes;
+          block_product(tmem + half * COLS, at, at + kRows * kRowBytes, instruction_descriptor_e4m3(COLS));
+          commit(empty + 8 * s);
+          commit(filled + 8 * half);
+        }
+      }
+      for (int last = max(0, step - 2); last < step; ++last)
+        if (!wait_bounded(filled + 8 * (last & 1), (last / 2) & 1)) healthy = false;
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    constexpr int kMine = COLS / 2;  // outputs of this warp's half
+    const int quarter = warp & 3, half_cols = (warp - 4) >> 2;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half_cols * kMine;
+    uint8_t* store = shared + kStages * S::kStageBytes + (warp - 4) * 32 * 128;
+    const int weight_rows = (out_features + kBlockK - 1) / kBlockK;
+    int step = 0;
+    for (int tile = blockIdx.x; tile < tiles && healthy; tile += gridDim.x) {
+      int row_tile, col_tile;
+      tile_at(tile, row_tile, col_tile);
+      const int token = row_tile * kRows + quarter * 32 + lane;
+      const int col0 = col_tile * COLS + half_cols * kMine;
+      // (a token or weight block past the end reads the last one's scale: its sums are not stored)
+      const float* sa_at = sa + min(token, tokens - 1);
+      const float* sw_at = sw + static_cast<size_t>(min(col0 / kBlockK, weight_rows - 1)) * blocks;
+      auto scale_at = [&](int b) {
+        const int at = min(b, blocks - 1);
+        return __fmul_rn(load_scale(sa_at + static_cast<size_t>(at) * tokens), load_scale(sw_at + at));
+      };
+      float sum[kMine];
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) sum[i] = 0.0f;
+      float scale = scale_at(0), next = scale_at(1);
+      for (int b = 0; b < blocks; ++b, ++step) {
+        const float after = scale_at(b + 2);  // requested two blocks ahead of its use
+        const int half = step & 1;
+        if (!(healthy = __all_sync(kFullMask, wait_bounded(filled + 8 * half, (step / 2) & 1)))) break;
+        fence_after_sync();
+        constexpr int kGroup = 16, kGroups = kMine / kGroup;
+        uint32_t d[2][kGroup];
+        load16(lane_base + half * COLS, d[0]);
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          wait_loads(d[g & 1]);
+          if (g + 1 < kGroups) {
+            load16(lane_base + half * COLS + (g + 1) * kGroup, d[(g + 1) & 1]);
+          } else {
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) barrier_arrive(drained + 8 * half);
+          }
+#pragma unroll
+          for (int i = 0; i < kGroup; i += 2) {
+            const int at = g * kGroup + i;
+            const float2 r = fma2(make_float2(scale, scale),
+                                  make_float2(__uint_as_float(d[g & 1][i]), __uint_as_float(d[g & 1][i + 1])),
+                                  make_float2(sum[at], sum[at + 1]));
+            sum[at] = r.x;
+            sum[at + 1] = r.y;
+          }
+        }
+        scale = next;
+        next = after;
+      }
+      if (!healthy) break;
+      // 32 rows x 64 outputs at a time through the warp's own 4 KB (swizzled like the copy reads it)
+#pragma unroll
+      for (int g = 0; g < kMine / 64; ++g) {
+        if (lane == 0) store_wait_read<0>();
+        __syncwarp();
+#pragma unroll
+        for (int piece = 0; piece < 8; ++piece) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = sum[g * 64 + piece * 8 + e];
+          *reinterpret_cast<uint4*>(store + lane * 128 + ((piece ^ (lane & 7)) << 4)) = pack8(v);
+        }
+        fence_async_proxy();
+        __syncwarp();
+        const int x = col0 + g * 64, y = row_tile * kRows + quarter * 32;
+        if (lane == 0 && x < out_features && y < tokens) {
+          store_box(&map_out, x, y, shared_address(store));
+          store_commit();
+        }
+      }
+    }
+    if (lane == 0) store_wait<0>();
+  }
+  if (!healthy) atomicExch(&g_error, 1u);
+  __syncwarp();
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 2)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * COLS) : "memory");
+}
+
+}  // namespace panel
+
+// ------------------------------------------------------------------------------------------------------------- strip
+namespace strip {
+
+constexpr int kRows = 128;     // outputs of a tile
+constexpr int kThreads = 192;  // warp 0 fetches, warp 1 issues and owns the tensor memory, 2 to 5 add up
+constexpr int kMaxSplits = 8;  // CTAs of a cluster, one share of K each
+
+template <int COLS>
+struct Shape {
+  static constexpr int kStageBytes = (kRows + COLS) * kRowBytes;
+  static constexpr int kCtasPerSm = COLS == 128 ? 1 : 2;
+  static constexpr int kStages = COLS == 16 ? 6 : COLS == 32 ? 5 : COLS == 64 ? 4 : 6;
+  static constexpr int kScales = kStages * kStageBytes;           // [2][COLS] products of the two scales
+  static constexpr int kBarriers = kScales + 2 * COLS * 4;
+  static constexpr int kShared = 1024 + kBarriers + 256;
+  static constexpr int kColumns = 2 * COLS < 32 ? 32 : 2 * COLS;  // of tensor memory
+  static_assert(COLS * kRows * 4 <= kStages * kStageBytes, "the partial sums reuse the stages");
+};
+
+// CTA (rank, output tile, token tile); the cluster's CTAs share the blocks of K of one tile and add their sums in rank
+// order, each an equal part of the tile, out of one another's shared memory.
+template <int COLS>
+__global__ void __launch_bounds__(kThreads, Shape<COLS>::kCtasPerSm)
+    block_gemm_strip_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+                            const float* __restrict__ sa, const float* __restrict__ sw, int tokens, int out_features, int blocks,
+                            uint16_t* __restrict__ out) {
+  using S = Shape<COLS>;
+  constexpr int kStages = S::kStages;
+  extern __shared__ uint8_t raw[];
+  uint8_t* shared = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const uint32_t base = shared_address(shared);
+  const uint32_t full = base + S::kBarriers, empty = full + 8 * kStages, filled = empty + 8 * kStages, drained = filled + 16;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(shared + S::kBarriers + 16 * kStages + 32);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int splits = gridDim.x, rank = blockIdx.x;
+  const int row0 = blockIdx.y * kRows, token0 = blockIdx.z * COLS;
+  const int first = static_cast<int>(static_cast<long long>(blocks) * rank / splits);
+  const int count = static_cast<int>(static_cast<long long>(blocks) * (rank + 1) / splits) - first;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      barrier_init(full + 8 * s, 1);
+      barrier_init(empty + 8 * s, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      barrier_init(filled + 8 * i, 1);
+      barrier_init(drained + 8 * i, 4);
+    }
+    barrier_init_fence();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(const_cast<uint32_t*>(tmem_slot))),
+                 "r"(S::kColumns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  // only now: a successor that took this SM's tensor memory first would wait for this kernel and this kernel for it
+  release_next_kernel();
+  wait_for_prior_kernels();
+
+  bool healthy = true;
+  float sum[COLS];  // (of the adding warps: this thread's output row, every token of the tile)
+#pragma unroll
+  for (int i = 0; i < COLS; ++i) sum[i] = 0.0f;
+  const int quarter = warp & 3, row = quarter * 32 + lane;
+  if (warp == 0) {
+    if (lane == 0) {
+      int step = 0;
+      for (; step < count; ++step) {
+        const int s = step % kStages;
+        if (step >= kStages && !(healthy = wait_bounded(empty + 8 * s, (step / kStages - 1) & 1))) break;
+        const uint32_t at = base + s * S::kStageBytes;
+        barrier_expect(full + 8 * s, S::kStageBytes);
+        load_box(at, &map_w, (first + step) * kBlockK, row0, full + 8 * s);
+        load_box(at + kRows * kRowBytes, &map_a, (first + step) * kBlockK, token0, full + 8 * s);
+      }
+      for (int last = max(0, step - kStages); last < step; ++last)
+        if (!wait_bounded(full + 8 * (last % kStages), (last / kStages) & 1)) healthy = false;
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int step = 0;
+      for (; step < count; ++step) {
+        const int s = step % kStages, half = step & 1;
+        if (step >= 2 && !(healthy = wait_bounded(drained + 8 * half, (step / 2 - 1) & 1))) break;
+        if (!(healthy = wait_bounded(full + 8 * s, (step / kStages) & 1))) break;
+        fence_after_sync();
+        const uint32_t at = base + s * S::kStageBytes;
+        block_product(tmem + half * COLS, at, at + kRows * kRowBytes, instruction_descriptor_e4m3(COLS));
+        commit(empty + 8 * s);
+        commit(filled + 8 * half);
+      }
+      for (int last = max(0, step - 2); last < step; ++last)
+        if (!wait_bounded(filled + 8 * (last & 1), (last / 2) & 1)) healthy = false;
+    }
+  } else {
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const int mine = threadIdx.x - 64;  // the token whose scale this thread fetches
+    const bool fetches = mine < COLS;
+    const int token = token0 + mine;
+    const float* sa_at = sa + min(token, tokens - 1);
+    const float* sw_at = sw + static_cast<size_t>(blockIdx.y) * blocks;
+    auto scale_at = [&](int b) {
+      const int at = first + min(b, count - 1);
+      return fetches && token < tokens ? __fmul_rn(load_scale(sa_at + static_cast<size_t>(at) * tokens), load_scale(sw_at + at)) : 0.0f;
+    };
+    float* scales = reinterpret_cast<float*>(shared + S::kScales);
+    float scale = scale_at(0), next = scale_at(1);
+    constexpr int kGroup = COLS < 32 ? COLS : (COLS == 128 ? 16 : 32);
+    for (int step = 0; step < count; ++step) {
+      const float after = scale_at(step + 2);
+      const int half = step & 1;
+      // the products of the block's scales, for everybody: written to the half that was read two steps ago
+      if (fetches) scales[half * COLS + mine] = scale;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      // (no way out of the loop: the other warps count on this one at the barrier above)
+      if (healthy) healthy = __all_sync(kFullMask, wait_bounded(filled + 8 * half, (step / 2) & 1));
+      fence_after_sync();
+      const float4* factors = reinterpret_cast<const float4*>(scales + half * COLS);
+#pragma unroll
+      for (int g = 0; g < COLS / kGroup; ++g) {
+        uint32_t d[kGroup];
+        if constexpr (kGroup == 16) load16(lane_base + half * COLS + g * kGroup, d);
+        else load32(lane_base + half * COLS + g * kGroup, d);
+        wait_loads(d);
+        if (g + 1 == COLS / kGroup) {
+          fence_before_sync();
+          __syncwarp();
+          if (lane == 0) barrier_arrive(drained + 8 * half);
+        }
+#pragma unroll
+        for (int i = 0; i < kGroup; i += 4) {
+          const float4 f = factors[(g * kGroup + i) / 4];
+          sum[g * kGroup + i] = fmaf(f.x, __uint_as_float(d[i]), sum[g * kGroup + i]);
+          sum[g * kGroup + i + 1] = fmaf(f.y, __uint_as_float(d[i + 1]), sum[g * kGroup + i + 1]);
+          sum[g * kGroup + i + 2] = fmaf(f.z, __uint_as_float(d[i + 2]), sum[g * kGroup + i + 2]);
+          sum[g * kGroup + i + 3] = fmaf(f.w, __uint_as_float(d[i + 3]), sum[g * kGroup + i + 3]);
+        }
+      }
+      scale = next;
+      next = after;
     }
   }
+  if (!healthy) atomicExch(&g_error, 1u);
+  __syncwarp();
+  fence_before_sync();
+  __syncthreads();  // every copy has landed and every product is complete: the stages are free
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kColumns) : "memory");
+  float* partial = reinterpret_cast<float*>(shared);  // [token][output row]
+  if (warp >= 2) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const size_t t = t0 + ty * 4 + i;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const size_t o = n0 + tx * 4 + j;
-      if (t < tokens && o < n) out[t * n + o] = float_to_bf16(total[i][j]);
+    for (int i = 0; i < COLS; ++i) partial[i * kRows + row] = sum[i];
+  }
+  // (all threads of all CTAs of the cluster come here, healthy or not)
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  // rank r finishes the items r, r + splits, ... of threads-many: item = (token, four outputs)
+  const int visible = min(COLS, tokens - token0);
+  for (int item = rank * kThreads + threadIdx.x; item < visible * (kRows / 4); item += splits * kThreads) {
+    const int t = item / (kRows / 4), r = (item % (kRows / 4)) * 4;
+    const uint32_t at = base + static_cast<uint32_t>((t * kRows + r) * 4);
+    float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int from = 0; from < splits; ++from) {
+      uint32_t there;
+      float4 p;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(from));
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(p.x), "=f"(p.y), "=f"(p.z), "=f"(p.w)
+                   : "r"(there)
+                   : "memory");
+      total.x += p.x;
+      total.y += p.y;
+      total.z += p.z;
+      total.w += p.w;
+    }
+    if (row0 + r < out_features)
+      *reinterpret_cast<uint2*>(out + static_cast<size_t>(token0 + t) * out_features + row0 + r) =
+          make_uint2(pack_bf16x2(total.x, total.y), pack_bf16x2(total.z, total.w));
+  }
+  // no CTA leaves while another may still read its sums
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+}  // namespace strip
+
+// ------------------------------------------------------------------------------------------------------------- host
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encoder() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// [rows, cols] row-major, boxes of box_rows rows of 128 bytes, swizzled; elements past the edges read as zero.
+bool encode_map(CUtensorMap* map, CUtensorMapDataType type, int element, const void* p, size_t rows, size_t cols, int box_rows) {
+  const EncodeTiled encode = encoder();
+  if (encode == nullptr) return false;
+  const cuuint64_t sizes[2] = {cols, rows}, strides[1] = {cols * element};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / element), static_cast<cuuint32_t>(box_rows)}, steps[2] = {1, 1};
+  return encode(map, type, 2, const_cast<void*>(p), sizes, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Opts a kernel in to its shared memory, once per device; `registers` (when not 0) is what the kernel's register split
+// was written for.
+template <auto kKernel>
+int prepare_kernel(int shared, int registers) {
+  static std::atomic<unsigned long long> ready{0};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const unsigned long long bit = 1ull << (device & 63);
+  if (ready.load(std::memory_order_acquire) & bit) return host::kOk;
+  if (registers != 0) {
+    cudaFuncAttributes attributes;
+    if ((e = cudaFuncGetAttributes(&attributes, kKernel)) != cudaSuccess) return static_cast<int>(e);
+    if (attributes.numRegs != registers) return host::kNotSupported;  // the split would wait for registers it never gets
+  }
+  if ((e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared)) != cudaSuccess)
+    return static_cast<int>(e);
+  ready.fetch_or(bit, std::memory_order_release);
+  return host::kOk;
+}
+
+struct Problem {
+  const uint8_t *weights, *activations;
+  const float *weight_scales, *activation_scales;
+  int tokens, out_features, in_features, blocks;
+  uint16_t* out;
+  cudaStream_t stream;
+};
+
+template <int COLS>
+int launch_panel(const Problem& p) {
+  using S = panel::Shape<COLS>;
+  constexpr auto kernel = panel::block_gemm_panel_kernel<COLS>;
+  const int status = prepare_kernel<kernel>(S::kShared, panel::kLaunchRegisters);
+  if (status != host::kOk) return status;
+  CUtensorMap a, w, o;
+  if (!encode_map(&a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.activations, p.tokens, p.in_features, panel::kRows) ||
+      !encode_map(&w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.weights, p.out_features, p.in_features, COLS) ||
+      !encode_map(&o, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.out, p.tokens, p.out_features, 32))
+    return host::kNotSupported;
+  const int row_tiles = (p.tokens + panel::kRows - 1) / panel::kRows, col_tiles = (p.out_features + COLS - 1) / COLS;
+  if (static_cast<long long>(row_tiles) * col_tiles > 0x7fffffff / 2) return host::kNotSupported;
+  const int tiles = row_tiles * col_tiles, sms = host::current_device_sm_count();
+  host::launch_kernel(kernel, dim3(tiles < sms ? tiles : sms), dim3(panel::kThreads), S::kShared, p.stream, true, a, w, o,
+                      p.activation_scales, p.weight_scales, p.tokens, p.out_features, p.blocks, row_tiles, col_tiles);
+  return host::launch_status();
+}
+
+// CTAs that share a tile's blocks of K: the count with the least time on the busiest SM, in blocks, plus what joining
+// the sums costs (measured as about two blocks).
+int strip_splits(int tiles, int blocks, int slots) {
+  int best = 1;
+  double least = 1e300;
+  for (int s = 1; s <= strip::kMaxSplits && s <= blocks; ++s) {
+    const double waves = (static_cast<long long>(tiles) * s + slots - 1) / slots;
+    const double time = waves * ((blocks + s - 1) / s) + (s > 1 ? 2.0 : 0.0);
+    if (time < least) {
+      least = time;
+      best = s;
     }
   }
+  return best;
+}
+
+template <int COLS>
+int launch_strip(const Problem& p) {
+  using S = strip::Shape<COLS>;
+  constexpr auto kernel = strip::block_gemm_strip_kernel<COLS>;
+  const int status = prepare_kernel<kernel>(S::kShared, 0);
+  if (status != host::kOk) return status;
+  CUtensorMap a, w;
+  if (!encode_map(&a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.activations, p.tokens, p.in_features, COLS) ||
+      !encode_map(&w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.weights, p.out_features, p.in_features, strip::kRows))
+    return host::kNotSupported;
+  const unsigned out_tiles = (p.out_features + strip::kRows - 1) / strip::kRows, token_tiles = (p.tokens + COLS - 1) / COLS;
+  if (out_tiles > 65535u || token_tiles > 65535u) return host::kNotSupported;
+  const int splits = strip_splits(static_cast<int>(out_tiles * token_tiles), p.blocks,
+                                  host::current_device_sm_count() * S::kCtasPerSm);
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(splits, out_tiles, token_tiles);
+  config.blockDim = dim3(strip::kThreads);
+  config.dynamicSmemBytes = S::kShared;
+  config.stream = p.stream;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeClusterDimension;
+  attributes[0].val.clusterDim.x = splits;
+  attributes[0].val.clusterDim.y = 1;
+  attributes[0].val.clusterDim.z = 1;
+  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attributes;
+  config.numAttrs = host::overlap_allowed() ? 2 : 1;
+  (void)cudaLaunchKernelEx(&config, kernel, a, w, p.activation_scales, p.weight_scales, p.tokens, p.out_features, p.blocks, p.out);
+  return host::launch_status();
 }
 
 }  // namespace
@@ -87,7 +565,9 @@ extern "C" int q3x_b200_fp8_block_gemm_bf16(const uint8_t* weights, const float*
                                             size_t in_features, uint16_t* out, void* stream) {
   if (tokens == 0 || out_features == 0) return kOk;
   if (in_features == 0 || in_features % 16 != 0 || out_features % 8 != 0) return kInvalid;
-  if (tokens > 0x7fffffffu || out_features > 0x7fffffffu || in_features > 0x7fffffffu) return kInvalid;
+  // (a tile's coordinates, one tile past the end included, are 32-bit integers)
+  constexpr size_t kMost = 0x7fffffffu - 256;
+  if (tokens > kMost || out_features > kMost || in_features > kMost) return kInvalid;
   if (weights == nullptr || weight_scales == nullptr || activations == nullptr || activation_scales == nullptr || out == nullptr)
     return kInvalid;
   const size_t blocks = (in_features + kBlockK - 1) / kBlockK;
@@ -101,11 +581,20 @@ extern "C" int q3x_b200_fp8_block_gemm_bf16(const uint8_t* weights, const float*
   if (!aligned16(weights) || !aligned16(activations) || !aligned16(out) ||
       (reinterpret_cast<uintptr_t>(weight_scales) & 3u) != 0 || (reinterpret_cast<uintptr_t>(activation_scales) & 3u) != 0)
     return kNotSupported;
-  const size_t token_tiles = (tokens + kTile - 1) / kTile, out_tiles = (out_features + kTile - 1) / kTile;
-  if (token_tiles > 65535u) return kNotSupported;
   clear_stale_error();
-  block_gemm_kernel<<<dim3(static_cast<unsigned>(out_tiles), static_cast<unsigned>(token_tiles)), kThreads, 0,
-                      as_stream(stream)>>>(weights, weight_scales, activations, activation_scales, tokens, out_features,
-                                           in_features, out);
-  return launch_status();
+  const Problem p{weights, activations, weight_scales, activation_scales, static_cast<int>(tokens), static_cast<int>(out_features),
+                  static_cast<int>(in_features), static_cast<int>(blocks), out, as_stream(stream)};
+  if (tokens <= 16) return launch_strip<16>(p);
+  if (tokens <= 32) return launch_strip<32>(p);
+  if (tokens <= 64) return launch_strip<64>(p);
+  if (tokens <= 128) return launch_strip<128>(p);
+  // 256 outputs per tile where that still gives every SM a tile
+  const size_t wide_tiles = (tokens + 127) / 128 * ((out_features + 255) / 256);
+  return wide_tiles >= static_cast<size_t>(current_device_sm_count()) ? launch_panel<256>(p) : launch_panel<128>(p);
+}
+
+extern "C" int q3x_b200_fp8_block_gemm_error(void) {
+  unsigned int word = 0;
+  if (cudaMemcpyFromSymbol(&word, g_error, sizeof(word)) != cudaSuccess) return -1;
+  return static_cast<int>(word);
 }

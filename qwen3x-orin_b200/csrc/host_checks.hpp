@@ -57,6 +57,12 @@ constexpr int kInvalid = static_cast<int>(cudaErrorInvalidValue);
 constexpr int kNotSupported = static_cast<int>(cudaErrorNotSupported);
 constexpr int kOk = static_cast<int>(cudaSuccess);
 
+// Q3X_B200_NO_OVERLAP=1 turns programmatic stream serialisation off for the whole process.
+inline bool overlap_allowed() {
+  static const bool allowed = std::getenv("Q3X_B200_NO_OVERLAP") == nullptr;
+  return allowed;
+}
+
 // Kernel launch with an explicit choice of programmatic stream serialisation: with `overlap` the kernel may
 // start before the previous kernel of the stream has finished (it must then call wait_for_prior_kernels()
 // before it touches global memory); without it this is the ordinary <<< >>> launch.  Works under stream
@@ -73,8 +79,7 @@ inline void launch_kernel(void (*kernel)(Params...), dim3 grid, dim3 block, size
   attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute[0].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attribute;
-  static const bool allowed = std::getenv("Q3X_B200_NO_OVERLAP") == nullptr;
-  config.numAttrs = overlap && allowed ? 1u : 0u;
+  config.numAttrs = overlap && overlap_allowed() ? 1u : 0u;
   (void)cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
 }
 

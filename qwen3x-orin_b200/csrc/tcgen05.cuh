@@ -1,7 +1,8 @@
 // The few tcgen05 (fifth-generation tensor core) building blocks the hand-written kernels here share: shared-memory
 // matrix descriptors for 128-byte-swizzled operands, the instruction descriptor of a bf16 x bf16 -> FP32 product with
 // M = 128, issue / commit, a BOUNDED wait on the completion barrier, tensor-memory loads and stores of a thread's own
-// lane, and the fences between the proxies.  Operand tiles are rows of 64 bf16 (128 bytes) whose 16-byte pieces are
+// lane, the fences between the proxies, and (for E4M3 operands fetched by bulk tensor copies) the matching instruction,
+// barriers and copies.  Operand tiles are rows of 64 bf16 (128 bytes) whose 16-byte pieces are
 // permuted by the row's low three bits -- the 128-byte swizzle -- in blocks whose base is 1024-byte aligned.
 #pragma once
 #include <cstdint>
@@ -88,6 +89,79 @@ __device__ __forceinline__ uint64_t operand_descriptor_mn(uint32_t shared_addres
          (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
 }
 constexpr uint32_t kBOperandMnMajor = 1u << 16;  // or-ed into an instruction descriptor
+
+// ---- E4M3 x E4M3 -> FP32 (32 elements of k per instruction; rows of 128 codes are the same 128 bytes as 64 bf16)
+__host__ __device__ constexpr uint32_t instruction_descriptor_e4m3(int n) {
+  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
+}
+__device__ __forceinline__ void mma_e4m3(uint32_t accumulator, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(accumulator),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// ---- barriers and bulk tensor copies
+__device__ __forceinline__ void barrier_init(uint32_t barrier, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(barrier), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_init_fence() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+__device__ __forceinline__ void barrier_expect(uint32_t barrier, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(uint32_t barrier) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(barrier) : "memory");
+}
+__device__ __forceinline__ bool barrier_try(uint32_t barrier, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(done)
+               : "r"(barrier), "r"(parity)
+               : "memory");
+  return done != 0;
+}
+// The bounded wait for kernels that wait once per tile of a long loop: the timer is only read after a thousand polls
+// (it costs more than a completed wait), and the bound is 200 ms.
+__device__ __forceinline__ bool wait_bounded(uint32_t barrier, uint32_t parity) {
+  for (int spin = 0; spin < 1024; ++spin)
+    if (barrier_try(barrier, parity)) return true;
+  uint64_t start, now;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
+  for (uint32_t spin = 0; spin < (1u << 28); ++spin) {
+    if (barrier_try(barrier, parity)) return true;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+    if (now - start > 200000000ull) return false;
+  }
+  return false;
+}
+// Box of a two-dimensional tensor map at (x, y) into this CTA's shared memory; completes `bytes` on the barrier.
+__device__ __forceinline__ void load_box(uint32_t shared_address, const void* map, int x, int y, uint32_t barrier) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                   shared_address),
+               "l"(map), "r"(x), "r"(y), "r"(barrier)
+               : "memory");
+}
+__device__ __forceinline__ void store_box(const void* map, int x, int y, uint32_t shared_address) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
+               "r"(shared_address)
+               : "memory");
+}
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// all but the newest N stores have read their shared memory / have completed
+template <int N>
+__device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+template <int N>
+__device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory"); }
+
+// wait_loads() that also names the registers waited for, so that no use of them can be scheduled in front of it
+__device__ __forceinline__ void wait_loads(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void wait_loads(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
 
 }  // namespace tcgen05
 }  // namespace q3x

@@ -136,13 +136,25 @@ def ptr(x):
     return int(x)
 
 
+_functions = {}  # name -> bound entry point
+_addressed = {int: False, float: False, type(None): False}  # argument type -> whether it has a device address
+
+
 def call(name: str, *args) -> int:
-    """Calls an entry point; tensor-likes are replaced by their device address."""
-    fn = getattr(lib(), name)
-    return fn(*[ptr(a) if (hasattr(a, "data_ptr") or a is None) else a for a in args])
+    """Calls an entry point; tensor-likes are replaced by their device address.  (A batch-one call is bound by what
+    happens here, so an entry point is looked up and an argument type asked once.)"""
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(lib(), name)
+    try:
+        return fn(*[a.data_ptr() if _addressed[a.__class__] else a for a in args])
+    except KeyError:  # a type not seen before
+        for a in args:
+            _addressed.setdefault(a.__class__, hasattr(a, "data_ptr"))
+    return fn(*[a.data_ptr() if _addressed[a.__class__] else a for a in args])
 
 
 def check(name: str, *args) -> None:
     st = call(name, *args)
-    if st != CUDA_SUCCESS:
+    if st:
         raise Q3xError(name, st)

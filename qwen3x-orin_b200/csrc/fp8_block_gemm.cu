@@ -38,6 +38,24 @@ __device__ __forceinline__ void block_product(uint32_t accumulator, uint32_t a, 
     mma_e4m3(accumulator, operand_descriptor(a + step * 32), operand_descriptor(b + step * 32), idesc, step > 0 ? 1u : 0u);
 }
 
+// One FP32 from global to shared memory; the lane's copies so far arrive on the barrier, which counts on that arrival,
+// when they have landed; and the wait for them at the end.
+__device__ __forceinline__ void copy_scale(uint32_t to, const float* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_arrive(uint32_t barrier) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(barrier) : "memory");
+}
+__device__ __forceinline__ float load_shared(uint32_t at) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// A bounded wait of a whole warp, with one answer for all its lanes.
+__device__ __forceinline__ bool wait_warp(uint32_t barrier, uint32_t parity) {
+  return __all_sync(kFullMask, barrier_try(barrier, parity)) || __all_sync(kFullMask, wait_bounded(barrier, parity));
+}
 // (volatile, unlike a read-only load: it must stay behind wait_for_prior_kernels())
 __device__ __forceinline__ float load_scale(const float* p) {
   float v;
@@ -50,26 +68,29 @@ __device__ __forceinline__ uint32_t shared_address(const void* p) { return stati
 namespace panel {
 
 constexpr int kRows = 128;                  // tokens of a tile
-constexpr int kThreads = 384;               // warp 0 fetches, warp 1 issues, warp 2 owns the tensor memory, 4 to 11 add up
+constexpr int kThreads = 384;               // warp 0 fetches codes, 2 scales, 1 and 3 issue, 4 to 11 add up
 constexpr int kAdders = 8;                  // warps: 4 lane quarters x 2 column halves
 constexpr int kLaunchRegisters = 168;       // 65536 / 384, rounded down to 8
+constexpr int kSlots = 8;                   // of scales, one per block in flight
+constexpr int kSlotFloats = kRows + 4;
 constexpr int kBand = 16;                   // token tiles walked together
 
 template <int COLS>
 struct Shape {
   static constexpr int kStageBytes = (kRows + COLS) * kRowBytes;
   static constexpr int kStages = COLS == 256 ? 4 : 6;
-  static constexpr int kStoreBytes = kAdders * 32 * 128;  // a warp's 32 rows x 64 outputs
-  static constexpr int kBarriers = kStages * kStageBytes + kStoreBytes;
+  static constexpr int kStore = kStages * kStageBytes;          // [adder][32 rows][32 outputs] bf16
+  static constexpr int kScales = kStore + kAdders * 32 * 64;    // [slot][128 tokens, 2 column halves, 2 unused] FP32
+  static constexpr int kBarriers = kScales + kSlots * kSlotFloats * 4;
   static constexpr int kShared = 1024 + kBarriers + 256;  // (1024: the stages start on a 1024-byte boundary)
+  static_assert(kStages + 2 <= kSlots, "see the warp that fetches scales");
 };
 
 template <int COLS>
 __global__ void __launch_bounds__(kThreads, 1)
     block_gemm_panel_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
-                            const __grid_constant__ CUtensorMap map_out, const float* __restrict__ sa,
-                            const float* __restrict__ sw, int tokens, int out_features, int blocks, int row_tiles,
-                            int col_tiles) {
+                            const float* __restrict__ sa, const float* __restrict__ sw, int tokens, int out_features,
+                            int blocks, int row_tiles, int col_tiles, uint16_t* __restrict__ out) {
   using S = Shape<COLS>;
   constexpr int kStages = S::kStages;
   extern __shared__ uint8_t raw[];
@@ -82,7 +103,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      barrier_init(full + 8 * s, 1);
+      barrier_init(full + 8 * s, 1 + 32);  // the codes' fetcher and every lane of the scales'
       barrier_init(empty + 8 * s, 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -117,118 +138,154 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool healthy = true;
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {
       int step = 0;
       for (int tile = blockIdx.x; tile < tiles && healthy; tile += gridDim.x) {
         int row_tile, col_tile;
         tile_at(tile, row_tile, col_tile);
         for (int b = 0; b < blocks; ++b, ++step) {
           const int s = step % kStages;
-          if (step >= kStages && !(healthy = wait_bounded(empty + 8 * s, (step / kStages - 1) & 1))) break;
+          if (step >= kStages && !(healthy = wait_warp(empty + 8 * s, (step / kStages - 1) & 1))) break;
           const uint32_t at = base + s * S::kStageBytes;
-          barrier_expect(full + 8 * s, S::kStageBytes);
-          load_box(at, &map_a, b * kBlockK, row_tile * kRows, full + 8 * s);
-          load_box(at + kRows * kRowBytes, &map_w, b * kBlockK, col_tile * COLS, full + 8 * s);
+          if (elect_one()) {
+            barrier_expect(full + 8 * s, S::kStageBytes);
+            load_box(at, &map_a, b * kBlockK, row_tile * kRows, full + 8 * s);
+            load_box(at + kRows * kRowBytes, &map_w, b * kBlockK, col_tile * COLS, full + 8 * s);
+          }
         }
       }
       // no copy is in flight when the CTA ends, whatever became of its readers
       for (int last = max(0, step - kStages); last < step; ++last)
-        if (!wait_bounded(full + 8 * (last % kStages), (last / kStages) & 1)) healthy = false;
-    } else if (warp == 1 && lane == 0) {
+        if (!wait_warp(full + 8 * (last % kStages), (last / kStages) & 1)) healthy = false;
+    } else if (warp == 2) {
+      // The scales of a block, copied without passing through registers (a load held in one for two blocks was measured to
+      // hold up the whole warp wherever the compiler moved it).  Slot t & 7 was last read for step t - 8: when step
+      // t - kStages has left its stage its accumulator was free, so step t - kStages - 2 and all before it were drained.
+      const int weight_rows = (out_features + kBlockK - 1) / kBlockK;
       int step = 0;
       for (int tile = blockIdx.x; tile < tiles && healthy; tile += gridDim.x) {
+        int row_tile, col_tile;
+        tile_at(tile, row_tile, col_tile);
+        const float* rows = sa + row_tile * kRows;
+        const int visible = min(kRows, tokens - row_tile * kRows);
+        // (a weight block past the end reads the last one's scale: its sums are not stored)
+        const int weight_row = min((col_tile * COLS + (lane & 1) * (COLS / 2)) / kBlockK, weight_rows - 1);
+        const float* weight = sw + static_cast<size_t>(weight_row) * blocks;
         for (int b = 0; b < blocks; ++b, ++step) {
-          const int s = step % kStages, half = step & 1;
-          if (step >= 2 && !(healthy = wait_bounded(drained + 8 * half, (step / 2 - 1) & 1))) break;
-          if (!(healthy = wait_bounded(full + 8 * s, (step / kStages) & 1))) break;
-          fence_after_sync();
-          const uint32_t at = base + s * S::kStageBytes;
+          const int s = step % kStages;
+          if (step >= kStages && !(healthy = wait_warp(empty + 8 * s, (step / kStages - 1) & 1))) break;
+          const uint32_t slot = base + S::kScales + (step % kSlots) * kSlotFloats * 4;
+#pragma unroll
+          for (int i = 0; i < kRows; i += 32) copy_scale(slot + (i + lane) * 4, rows + min(i + lane, visible - 1));
+          if (lane < 2) copy_scale(slot + (kRows + lane) * 4, weight + b);
+          copies_arrive(full + 8 * s);
+          rows += tokens;
+        }
+      }
+      copies_wait();
+    } else {
+      // Warp 1 issues the even steps, warp 3 the odd ones.  A warp's instructions wait in line behind its own products, so
+      // one warp alone would test the next step's barriers only once its products are in the pipe, and the pipe would run
+      // dry for the time of those tests (measured: 900 cycles per block instead of 512).
+      const int half = warp >> 1, steps = (tiles - static_cast<int>(blockIdx.x) + gridDim.x - 1) / gridDim.x * blocks;
+      int step = half;
+      for (; step < steps; step += 2) {
+        const int s = step % kStages;
+        if (!(healthy = wait_warp(full + 8 * s, (step / kStages) & 1))) break;
+        if (step >= 2 && !(healthy = wait_warp(drained + 8 * half, (step / 2 - 1) & 1))) break;
+        fence_after_sync();
+        const uint32_t at = base + s * S::kStageBytes;
+        if (elect_one()) {
           block_product(tmem + half * COLS, at, at + kRows * kRowBytes, instruction_descriptor_e4m3(COLS));
           commit(empty + 8 * s);
           commit(filled + 8 * half);
         }
+        __syncwarp();
       }
-      for (int last = max(0, step - 2); last < step; ++last)
-        if (!wait_bounded(filled + 8 * (last & 1), (last / 2) & 1)) healthy = false;
+      if (step >= 2 && !wait_warp(filled + 8 * half, (step / 2 - 1) & 1)) healthy = false;
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     constexpr int kMine = COLS / 2;  // outputs of this warp's half
     const int quarter = warp & 3, half_cols = (warp - 4) >> 2;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half_cols * kMine;
-    uint8_t* store = shared + kStages * S::kStageBytes + (warp - 4) * 32 * 128;
-    const int weight_rows = (out_features + kBlockK - 1) / kBlockK;
+    uint8_t* store = shared + S::kStore + (warp - 4) * 32 * 64;
+    const uint32_t row_scale = base + S::kScales + (quarter * 32 + lane) * 4, col_scale = base + S::kScales + (kRows + half_cols) * 4;
     int step = 0;
     for (int tile = blockIdx.x; tile < tiles && healthy; tile += gridDim.x) {
-      int row_tile, col_tile;
-      tile_at(tile, row_tile, col_tile);
-      const int token = row_tile * kRows + quarter * 32 + lane;
-      const int col0 = col_tile * COLS + half_cols * kMine;
-      // (a token or weight block past the end reads the last one's scale: its sums are not stored)
-      const float* sa_at = sa + min(token, tokens - 1);
-      const float* sw_at = sw + static_cast<size_t>(min(col0 / kBlockK, weight_rows - 1)) * blocks;
-      auto scale_at = [&](int b) {
-        const int at = min(b, blocks - 1);
-        return __fmul_rn(load_scale(sa_at + static_cast<size_t>(at) * tokens), load_scale(sw_at + at));
-      };
       float sum[kMine];
 #pragma unroll
       for (int i = 0; i < kMine; ++i) sum[i] = 0.0f;
-      float scale = scale_at(0), next = scale_at(1);
-      for (int b = 0; b < blocks; ++b, ++step) {
-        const float after = scale_at(b + 2);  // requested two blocks ahead of its use
-        const int half = step & 1;
-        if (!(healthy = __all_sync(kFullMask, wait_bounded(filled + 8 * half, (step / 2) & 1)))) break;
+      // One block: 32 columns of its accumulator at a time, times its scales, onto the sums; the next 32 columns, which may
+      // be the next block's first, are on their way meanwhile.
+      // Whether its products are complete is asked before the last columns but one are added and answered after.
+      uint32_t d[2][32];
+      float2 factors;
+      auto begin = [&](int at) {  // a block whose products are complete
         fence_after_sync();
-        constexpr int kGroup = 16, kGroups = kMine / kGroup;
-        uint32_t d[2][kGroup];
-        load16(lane_base + half * COLS, d[0]);
+        load32(lane_base + (at & 1) * COLS, d[0]);
+        factors = make_float2(load_shared(row_scale + at % kSlots * (kSlotFloats * 4)),
+                              load_shared(col_scale + at % kSlots * (kSlotFloats * 4)));
+      };
+      bool begun = false;
+      for (int b = 0; b < blocks; ++b) {
+        if (!begun) {
+          if (!(healthy = wait_warp(filled + 8 * (step & 1), (step / 2) & 1))) break;
+          begin(step);
+        }
+        const uint32_t columns = lane_base + (step & 1) * COLS;
+        const float scale = __fmul_rn(factors.x, factors.y);
+        bool complete = false;
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
+        for (int g = 0; g < kMine / 32; ++g) {
           wait_loads(d[g & 1]);
-          if (g + 1 < kGroups) {
-            load16(lane_base + half * COLS + (g + 1) * kGroup, d[(g + 1) & 1]);
+          if (g + 1 < kMine / 32) {
+            load32(columns + (g + 1) * 32, d[(g + 1) & 1]);
+            if (g + 2 == kMine / 32) complete = barrier_try(filled + 8 * (~step & 1), ((step + 1) / 2) & 1);
           } else {
             fence_before_sync();
             __syncwarp();
-            if (lane == 0) barrier_arrive(drained + 8 * half);
+            if (lane == 0) barrier_arrive(drained + 8 * (step & 1));
+            ++step;
+            begun = b + 1 < blocks && __all_sync(kFullMask, complete);
+            if (begun) begin(step);
           }
 #pragma unroll
-          for (int i = 0; i < kGroup; i += 2) {
-            const int at = g * kGroup + i;
+          for (int i = 0; i < 32; i += 2) {
             const float2 r = fma2(make_float2(scale, scale),
                                   make_float2(__uint_as_float(d[g & 1][i]), __uint_as_float(d[g & 1][i + 1])),
-                                  make_float2(sum[at], sum[at + 1]));
-            sum[at] = r.x;
-            sum[at + 1] = r.y;
+                                  make_float2(sum[g * 32 + i], sum[g * 32 + i + 1]));
+            sum[g * 32 + i] = r.x;
+            sum[g * 32 + i + 1] = r.y;
           }
         }
-        scale = next;
-        next = after;
       }
       if (!healthy) break;
-      // 32 rows x 64 outputs at a time through the warp's own 4 KB (swizzled like the copy reads it)
+      int row_tile, col_tile;
+      tile_at(tile, row_tile, col_tile);
+      const int row0 = row_tile * kRows + quarter * 32, col0 = col_tile * COLS + half_cols * kMine;
+      // 32 rows x 32 outputs at a time through the warp's own 2 KB, so that a store covers whole 64-byte pieces of eight
+      // rows (16-byte parts permuted by the row: free of bank conflicts both ways)
 #pragma unroll
-      for (int g = 0; g < kMine / 64; ++g) {
-        if (lane == 0) store_wait_read<0>();
-        __syncwarp();
+      for (int g = 0; g < kMine / 32; ++g) {
 #pragma unroll
-        for (int piece = 0; piece < 8; ++piece) {
+        for (int part = 0; part < 4; ++part) {
           float v[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = sum[g * 64 + piece * 8 + e];
-          *reinterpret_cast<uint4*>(store + lane * 128 + ((piece ^ (lane & 7)) << 4)) = pack8(v);
+          for (int e = 0; e < 8; ++e) v[e] = sum[g * 32 + part * 8 + e];
+          st_vec(store + lane * 64 + ((part ^ ((lane >> 1) & 3)) << 4), pack8(v));
         }
-        fence_async_proxy();
         __syncwarp();
-        const int x = col0 + g * 64, y = row_tile * kRows + quarter * 32;
-        if (lane == 0 && x < out_features && y < tokens) {
-          store_box(&map_out, x, y, shared_address(store));
-          store_commit();
+        const int col = col0 + g * 32 + (lane & 3) * 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = i * 8 + (lane >> 2), t = row0 + r;
+          const uint4 v = ld_vec(store + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
+          if (t < tokens && col < out_features) st_vec(out + static_cast<size_t>(t) * out_features + col, v);
         }
+        __syncwarp();
       }
     }
-    if (lane == 0) store_wait<0>();
   }
   if (!healthy) atomicExch(&g_error, 1u);
   __syncwarp();
@@ -310,35 +367,36 @@ __global__ void __launch_bounds__(kThreads, Shape<COLS>::kCtasPerSm)
   for (int i = 0; i < COLS; ++i) sum[i] = 0.0f;
   const int quarter = warp & 3, row = quarter * 32 + lane;
   if (warp == 0) {
-    if (lane == 0) {
-      int step = 0;
-      for (; step < count; ++step) {
-        const int s = step % kStages;
-        if (step >= kStages && !(healthy = wait_bounded(empty + 8 * s, (step / kStages - 1) & 1))) break;
-        const uint32_t at = base + s * S::kStageBytes;
+    int step = 0;
+    for (; step < count; ++step) {
+      const int s = step % kStages;
+      if (step >= kStages && !(healthy = wait_warp(empty + 8 * s, (step / kStages - 1) & 1))) break;
+      const uint32_t at = base + s * S::kStageBytes;
+      if (elect_one()) {
         barrier_expect(full + 8 * s, S::kStageBytes);
         load_box(at, &map_w, (first + step) * kBlockK, row0, full + 8 * s);
         load_box(at + kRows * kRowBytes, &map_a, (first + step) * kBlockK, token0, full + 8 * s);
       }
-      for (int last = max(0, step - kStages); last < step; ++last)
-        if (!wait_bounded(full + 8 * (last % kStages), (last / kStages) & 1)) healthy = false;
     }
+    for (int last = max(0, step - kStages); last < step; ++last)
+      if (!wait_warp(full + 8 * (last % kStages), (last / kStages) & 1)) healthy = false;
   } else if (warp == 1) {
-    if (lane == 0) {
-      int step = 0;
-      for (; step < count; ++step) {
-        const int s = step % kStages, half = step & 1;
-        if (step >= 2 && !(healthy = wait_bounded(drained + 8 * half, (step / 2 - 1) & 1))) break;
-        if (!(healthy = wait_bounded(full + 8 * s, (step / kStages) & 1))) break;
-        fence_after_sync();
-        const uint32_t at = base + s * S::kStageBytes;
+    int step = 0;
+    for (; step < count; ++step) {
+      const int s = step % kStages, half = step & 1;
+      if (step >= 2 && !(healthy = wait_warp(drained + 8 * half, (step / 2 - 1) & 1))) break;
+      if (!(healthy = wait_warp(full + 8 * s, (step / kStages) & 1))) break;
+      fence_after_sync();
+      const uint32_t at = base + s * S::kStageBytes;
+      if (elect_one()) {
         block_product(tmem + half * COLS, at, at + kRows * kRowBytes, instruction_descriptor_e4m3(COLS));
         commit(empty + 8 * s);
         commit(filled + 8 * half);
       }
-      for (int last = max(0, step - 2); last < step; ++last)
-        if (!wait_bounded(filled + 8 * (last & 1), (last / 2) & 1)) healthy = false;
+      __syncwarp();
     }
+    for (int last = max(0, step - 2); last < step; ++last)
+      if (!wait_warp(filled + 8 * (last & 1), (last / 2) & 1)) healthy = false;
   } else {
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const int mine = threadIdx.x - 64;  // the token whose scale this thread fetches
@@ -346,23 +404,23 @@ __global__ void __launch_bounds__(kThreads, Shape<COLS>::kCtasPerSm)
     const int token = token0 + mine;
     const float* sa_at = sa + min(token, tokens - 1);
     const float* sw_at = sw + static_cast<size_t>(blockIdx.y) * blocks;
-    auto scale_at = [&](int b) {
+    auto factors_at = [&](int b) {
       const int at = first + min(b, count - 1);
-      return fetches && token < tokens ? __fmul_rn(load_scale(sa_at + static_cast<size_t>(at) * tokens), load_scale(sw_at + at)) : 0.0f;
+      return make_float2(load_scale(sa_at + static_cast<size_t>(at) * tokens), load_scale(sw_at + at));
     };
     float* scales = reinterpret_cast<float*>(shared + S::kScales);
-    float scale = scale_at(0), next = scale_at(1);
     constexpr int kGroup = COLS < 32 ? COLS : (COLS == 128 ? 16 : 32);
-    for (int step = 0; step < count; ++step) {
-      const float after = scale_at(step + 2);
+    int step = 0;
+    auto add_block = [&](float2& factors, int b) {  // (two sets of factors that stay in their registers, as above)
       const int half = step & 1;
       // the products of the block's scales, for everybody: written to the half that was read two steps ago
-      if (fetches) scales[half * COLS + mine] = scale;
+      if (fetches) scales[half * COLS + mine] = token < tokens ? __fmul_rn(factors.x, factors.y) : 0.0f;
+      factors = factors_at(b + 2);
       asm volatile("bar.sync 1, 128;" ::: "memory");
       // (no way out of the loop: the other warps count on this one at the barrier above)
-      if (healthy) healthy = __all_sync(kFullMask, wait_bounded(filled + 8 * half, (step / 2) & 1));
+      if (healthy) healthy = wait_warp(filled + 8 * half, (step / 2) & 1);
       fence_after_sync();
-      const float4* factors = reinterpret_cast<const float4*>(scales + half * COLS);
+      const float4* scale4 = reinterpret_cast<const float4*>(scales + half * COLS);
 #pragma unroll
       for (int g = 0; g < COLS / kGroup; ++g) {
         uint32_t d[kGroup];
@@ -376,15 +434,20 @@ __global__ void __launch_bounds__(kThreads, Shape<COLS>::kCtasPerSm)
         }
 #pragma unroll
         for (int i = 0; i < kGroup; i += 4) {
-          const float4 f = factors[(g * kGroup + i) / 4];
-          sum[g * kGroup + i] = fmaf(f.x, __uint_as_float(d[i]), sum[g * kGroup + i]);
-          sum[g * kGroup + i + 1] = fmaf(f.y, __uint_as_float(d[i + 1]), sum[g * kGroup + i + 1]);
-          sum[g * kGroup + i + 2] = fmaf(f.z, __uint_as_float(d[i + 2]), sum[g * kGroup + i + 2]);
-          sum[g * kGroup + i + 3] = fmaf(f.w, __uint_as_float(d[i + 3]), sum[g * kGroup + i + 3]);
+          const float4 f = scale4[(g * kGroup + i) / 4];
+          float* to = sum + g * kGroup + i;
+          to[0] = fmaf(f.x, __uint_as_float(d[i]), to[0]);
+          to[1] = fmaf(f.y, __uint_as_float(d[i + 1]), to[1]);
+          to[2] = fmaf(f.z, __uint_as_float(d[i + 2]), to[2]);
+          to[3] = fmaf(f.w, __uint_as_float(d[i + 3]), to[3]);
         }
       }
-      scale = next;
-      next = after;
+      ++step;
+    };
+    float2 even = factors_at(0), odd = factors_at(1);
+    for (int b = 0; b < count; b += 2) {
+      add_block(even, b);
+      if (b + 1 < count) add_block(odd, b + 1);
     }
   }
   if (!healthy) atomicExch(&g_error, 1u);
@@ -448,14 +511,15 @@ EncodeTiled encoder() {
   return fn;
 }
 
-// [rows, cols] row-major, boxes of box_rows rows of 128 bytes, swizzled; elements past the edges read as zero.
-bool encode_map(CUtensorMap* map, CUtensorMapDataType type, int element, const void* p, size_t rows, size_t cols, int box_rows) {
+// Codes [rows, cols] in boxes of box_rows rows of 128, swizzled; past the edges they read as zero.
+bool encode_map(CUtensorMap* map, const uint8_t* codes, size_t rows, size_t cols, int box_rows) {
   const EncodeTiled encode = encoder();
   if (encode == nullptr) return false;
-  const cuuint64_t sizes[2] = {cols, rows}, strides[1] = {cols * element};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / element), static_cast<cuuint32_t>(box_rows)}, steps[2] = {1, 1};
-  return encode(map, type, 2, const_cast<void*>(p), sizes, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const cuuint64_t sizes[2] = {cols, rows}, strides[1] = {cols};
+  const cuuint32_t box[2] = {kRowBytes, static_cast<cuuint32_t>(box_rows)}, steps[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), sizes, strides, box, steps,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Opts a kernel in to its shared memory, once per device; `registers` (when not 0) is what the kernel's register split
@@ -493,16 +557,15 @@ int launch_panel(const Problem& p) {
   constexpr auto kernel = panel::block_gemm_panel_kernel<COLS>;
   const int status = prepare_kernel<kernel>(S::kShared, panel::kLaunchRegisters);
   if (status != host::kOk) return status;
-  CUtensorMap a, w, o;
-  if (!encode_map(&a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.activations, p.tokens, p.in_features, panel::kRows) ||
-      !encode_map(&w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.weights, p.out_features, p.in_features, COLS) ||
-      !encode_map(&o, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.out, p.tokens, p.out_features, 32))
+  CUtensorMap a, w;
+  if (!encode_map(&a, p.activations, p.tokens, p.in_features, panel::kRows) ||
+      !encode_map(&w, p.weights, p.out_features, p.in_features, COLS))
     return host::kNotSupported;
   const int row_tiles = (p.tokens + panel::kRows - 1) / panel::kRows, col_tiles = (p.out_features + COLS - 1) / COLS;
   if (static_cast<long long>(row_tiles) * col_tiles > 0x7fffffff / 2) return host::kNotSupported;
   const int tiles = row_tiles * col_tiles, sms = host::current_device_sm_count();
-  host::launch_kernel(kernel, dim3(tiles < sms ? tiles : sms), dim3(panel::kThreads), S::kShared, p.stream, true, a, w, o,
-                      p.activation_scales, p.weight_scales, p.tokens, p.out_features, p.blocks, row_tiles, col_tiles);
+  host::launch_kernel(kernel, dim3(tiles < sms ? tiles : sms), dim3(panel::kThreads), S::kShared, p.stream, true, a, w,
+                      p.activation_scales, p.weight_scales, p.tokens, p.out_features, p.blocks, row_tiles, col_tiles, p.out);
   return host::launch_status();
 }
 
@@ -529,8 +592,8 @@ int launch_strip(const Problem& p) {
   const int status = prepare_kernel<kernel>(S::kShared, 0);
   if (status != host::kOk) return status;
   CUtensorMap a, w;
-  if (!encode_map(&a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.activations, p.tokens, p.in_features, COLS) ||
-      !encode_map(&w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.weights, p.out_features, p.in_features, strip::kRows))
+  if (!encode_map(&a, p.activations, p.tokens, p.in_features, COLS) ||
+      !encode_map(&w, p.weights, p.out_features, p.in_features, strip::kRows))
     return host::kNotSupported;
   const unsigned out_tiles = (p.out_features + strip::kRows - 1) / strip::kRows, token_tiles = (p.tokens + COLS - 1) / COLS;
   if (out_tiles > 65535u || token_tiles > 65535u) return host::kNotSupported;

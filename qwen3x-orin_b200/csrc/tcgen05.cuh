@@ -101,6 +101,15 @@ __device__ __forceinline__ void mma_e4m3(uint32_t accumulator, uint64_t a, uint6
       : "memory");
 }
 
+// One lane of a converged warp, always the same one.  A warp that issues walks its loop with all lanes and lets this one
+// issue: addresses and descriptors then stay warp-uniform, which is what the tensor instructions take (a loop entered by
+// one lane alone moves every one of them into uniform registers again, a hundred cycles per instruction).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t elected;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected)::"memory");
+  return elected != 0;
+}
+
 // ---- barriers and bulk tensor copies
 __device__ __forceinline__ void barrier_init(uint32_t barrier, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(barrier), "r"(count) : "memory");

@@ -38,6 +38,27 @@ __device__ __forceinline__ void block_product(uint32_t accumulator, uint32_t a, 
     mma_e4m3(accumulator, operand_descriptor(a + step * 32), operand_descriptor(b + step * 32), idesc, step > 0 ? 1u : 0u);
 }
 
+// The cluster: a barrier of all its threads, an arrival on a rank's copy of a barrier, a rank's copy of four floats, and the
+// bounded wait for arrivals from other CTAs.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t at_rank(uint32_t address, int rank) {
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(address), "r"(rank));
+  return there;
+}
+__device__ __forceinline__ void arrive_at(uint32_t barrier, int rank) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at_rank(barrier, rank)) : "memory");
+}
+__device__ __forceinline__ float4 load_from(uint32_t address, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(at_rank(address, rank))
+               : "memory");
+  return v;
+}
 // One FP32 from global to shared memory; the lane's copies so far arrive on the barrier, which counts on that arrival,
 // when they have landed; and the wait for them at the end.
 __device__ __forceinline__ void copy_scale(uint32_t to, const float* from) {
@@ -56,11 +77,10 @@ __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;
 __device__ __forceinline__ bool wait_warp(uint32_t barrier, uint32_t parity) {
   return __all_sync(kFullMask, barrier_try(barrier, parity)) || __all_sync(kFullMask, wait_bounded(barrier, parity));
 }
-// (volatile, unlike a read-only load: it must stay behind wait_for_prior_kernels())
-__device__ __forceinline__ float load_scale(const float* p) {
-  float v;
-  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
-  return v;
+__device__ __forceinline__ bool wait_cluster(uint32_t barrier, uint32_t parity) {
+  const bool done = wait_warp(barrier, parity);
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+  return done;
 }
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
@@ -102,6 +122,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tiles = row_tiles * col_tiles;
 
   if (threadIdx.x == 0) {
+    prefetch_map(&map_a);
+    prefetch_map(&map_w);
     for (int s = 0; s < kStages; ++s) {
       barrier_init(full + 8 * s, 1 + 32);  // the codes' fetcher and every lane of the scales'
       barrier_init(empty + 8 * s, 1);
@@ -301,53 +323,65 @@ __global__ void __launch_bounds__(kThreads, 1)
 namespace strip {
 
 constexpr int kRows = 128;     // outputs of a tile
-constexpr int kThreads = 192;  // warp 0 fetches, warp 1 issues and owns the tensor memory, 2 to 5 add up
 constexpr int kMaxSplits = 8;  // CTAs of a cluster, one share of K each
 
+// Warp 0 fetches codes, 2 scales, 1 and 3 issue; the others add up: four for the four quarters of the lanes, and from 64
+// tokens on four more for the upper half of the tokens (128 tokens in one thread's registers: 57 us for 34816 x 5120,
+// bound by the additions).
 template <int COLS>
 struct Shape {
+  static constexpr int kAdders = COLS >= 64 ? 8 : 4;
+  static constexpr int kMine = COLS / (kAdders / 4);              // tokens of one adding warp
+  static constexpr int kThreads = 128 + 32 * kAdders;
   static constexpr int kStageBytes = (kRows + COLS) * kRowBytes;
-  static constexpr int kCtasPerSm = COLS == 128 ? 1 : 2;
-  static constexpr int kStages = COLS == 16 ? 6 : COLS == 32 ? 5 : COLS == 64 ? 4 : 6;
-  static constexpr int kScales = kStages * kStageBytes;           // [2][COLS] products of the two scales
-  static constexpr int kBarriers = kScales + 2 * COLS * 4;
+  static constexpr int kStages = COLS == 16 ? 11 : COLS == 32 ? 10 : COLS == 64 ? 7 : 4;
+  static constexpr int kSlots = COLS == 128 ? 8 : 16;             // of scales, one per block in flight
+  static constexpr int kSlotFloats = COLS + 4;                    // the tokens' scales, the weight block's, 3 unused
+  static constexpr int kPartial = kStages * kStageBytes;          // [token][output row] FP32, read by the whole cluster
+  static constexpr int kScales = kPartial + COLS * kRows * 4;
+  static constexpr int kBarriers = kScales + kSlots * kSlotFloats * 4;
   static constexpr int kShared = 1024 + kBarriers + 256;
-  static constexpr int kColumns = 2 * COLS < 32 ? 32 : 2 * COLS;  // of tensor memory
-  static_assert(COLS * kRows * 4 <= kStages * kStageBytes, "the partial sums reuse the stages");
+  static constexpr int kColumns = 2 * COLS;                       // of tensor memory
+  static_assert(kStages + 2 <= kSlots, "a slot is free when the step a ring of stages earlier has left its stage");
+  static_assert(16 * kStages + 52 <= 256 && kShared <= 232448, "shared memory of one CTA");
 };
 
-// CTA (rank, output tile, token tile); the cluster's CTAs share the blocks of K of one tile and add their sums in rank
-// order, each an equal part of the tile, out of one another's shared memory.
+// The cluster's CTAs share the blocks of K of one tile and add their sums in rank order, each an equal part of the tile,
+// out of one another's shared memory; then the cluster's next tile.
 template <int COLS>
-__global__ void __launch_bounds__(kThreads, Shape<COLS>::kCtasPerSm)
+__global__ void __launch_bounds__(Shape<COLS>::kThreads, 1)
     block_gemm_strip_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                             const float* __restrict__ sa, const float* __restrict__ sw, int tokens, int out_features, int blocks,
-                            uint16_t* __restrict__ out) {
+                            int token_tiles, int tiles, int splits, uint16_t* __restrict__ out) {
   using S = Shape<COLS>;
   constexpr int kStages = S::kStages;
   extern __shared__ uint8_t raw[];
   uint8_t* shared = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const uint32_t base = shared_address(shared);
-  const uint32_t full = base + S::kBarriers, empty = full + 8 * kStages, filled = empty + 8 * kStages, drained = filled + 16;
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(shared + S::kBarriers + 16 * kStages + 32);
+  const uint32_t full = base + S::kBarriers, empty = full + 8 * kStages, filled = empty + 8 * kStages, drained = filled + 16,
+                 ready = drained + 16, released = ready + 8;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(shared + S::kBarriers + 16 * kStages + 48);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int splits = gridDim.x, rank = blockIdx.x;
-  const int row0 = blockIdx.y * kRows, token0 = blockIdx.z * COLS;
+  const int rank = blockIdx.x % splits, cluster = blockIdx.x / splits, clusters = gridDim.x / splits;
   const int first = static_cast<int>(static_cast<long long>(blocks) * rank / splits);
   const int count = static_cast<int>(static_cast<long long>(blocks) * (rank + 1) / splits) - first;
 
   if (threadIdx.x == 0) {
+    prefetch_map(&map_a);
+    prefetch_map(&map_w);
     for (int s = 0; s < kStages; ++s) {
-      barrier_init(full + 8 * s, 1);
+      barrier_init(full + 8 * s, 1 + 32);  // the codes' fetcher and every lane of the scales'
       barrier_init(empty + 8 * s, 1);
     }
     for (int i = 0; i < 2; ++i) {
       barrier_init(filled + 8 * i, 1);
-      barrier_init(drained + 8 * i, 4);
+      barrier_init(drained + 8 * i, S::kAdders);
     }
+    barrier_init(ready, S::kAdders * splits);
+    barrier_init(released, S::kAdders * splits);
     barrier_init_fence();
   }
-  if (warp == 1) {
+  if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(const_cast<uint32_t*>(tmem_slot))),
                  "r"(S::kColumns)
                  : "memory");
@@ -355,6 +389,7 @@ __global__ void __launch_bounds__(kThreads, Shape<COLS>::kCtasPerSm)
   }
   fence_before_sync();
   __syncthreads();
+  cluster_sync();  // every CTA's barriers exist before another CTA arrives on them
   fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   // only now: a successor that took this SM's tensor memory first would wait for this kernel and this kernel for it
@@ -362,30 +397,31 @@ __global__ void __launch_bounds__(kThreads, Shape<COLS>::kCtasPerSm)
   wait_for_prior_kernels();
 
   bool healthy = true;
-  float sum[COLS];  // (of the adding warps: this thread's output row, every token of the tile)
-#pragma unroll
-  for (int i = 0; i < COLS; ++i) sum[i] = 0.0f;
-  const int quarter = warp & 3, row = quarter * 32 + lane;
   if (warp == 0) {
     int step = 0;
-    for (; step < count; ++step) {
-      const int s = step % kStages;
-      if (step >= kStages && !(healthy = wait_warp(empty + 8 * s, (step / kStages - 1) & 1))) break;
-      const uint32_t at = base + s * S::kStageBytes;
-      if (elect_one()) {
-        barrier_expect(full + 8 * s, S::kStageBytes);
-        load_box(at, &map_w, (first + step) * kBlockK, row0, full + 8 * s);
-        load_box(at + kRows * kRowBytes, &map_a, (first + step) * kBlockK, token0, full + 8 * s);
+    for (int tile = cluster; tile < tiles && healthy; tile += clusters) {
+      const int row0 = tile / token_tiles * kRows, token0 = tile % token_tiles * COLS;
+      for (int b = first; b < first + count; ++b, ++step) {
+        const int s = step % kStages;
+        if (step >= kStages && !(healthy = wait_warp(empty + 8 * s, (step / kStages - 1) & 1))) break;
+        const uint32_t at = base + s * S::kStageBytes;
+        if (elect_one()) {
+          barrier_expect(full + 8 * s, S::kStageBytes);
+          load_box(at, &map_w, b * kBlockK, row0, full + 8 * s);
+          load_box(at + kRows * kRowBytes, &map_a, b * kBlockK, token0, full + 8 * s);
+        }
       }
     }
+    // no copy is in flight when the CTA ends, whatever became of its readers
     for (int last = max(0, step - kStages); last < step; ++last)
       if (!wait_warp(full + 8 * (last % kStages), (last / kStages) & 1)) healthy = false;
-  } else if (warp == 1) {
-    int step = 0;
-    for (; step < count; ++step) {
-      const int s = step % kStages, half = step & 1;
-      if (step >= 2 && !(healthy = wait_warp(drained + 8 * half, (step / 2 - 1) & 1))) break;
+  } else if (warp == 1 || warp == 3) {  // even and odd steps, as in the panel kernel
+    const int half = warp >> 1, steps = (tiles - cluster + clusters - 1) / clusters * count;
+    int step = half;
+    for (; step < steps; step += 2) {
+      const int s = step % kStages;
       if (!(healthy = wait_warp(full + 8 * s, (step / kStages) & 1))) break;
+      if (step >= 2 && !(healthy = wait_warp(drained + 8 * half, (step / 2 - 1) & 1))) break;
       fence_after_sync();
       const uint32_t at = base + s * S::kStageBytes;
       if (elect_one()) {
@@ -395,100 +431,102 @@ __global__ void __launch_bounds__(kThreads, Shape<COLS>::kCtasPerSm)
       }
       __syncwarp();
     }
-    for (int last = max(0, step - 2); last < step; ++last)
-      if (!wait_warp(filled + 8 * (last & 1), (last / 2) & 1)) healthy = false;
-  } else {
-    const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    const int mine = threadIdx.x - 64;  // the token whose scale this thread fetches
-    const bool fetches = mine < COLS;
-    const int token = token0 + mine;
-    const float* sa_at = sa + min(token, tokens - 1);
-    const float* sw_at = sw + static_cast<size_t>(blockIdx.y) * blocks;
-    auto factors_at = [&](int b) {
-      const int at = first + min(b, count - 1);
-      return make_float2(load_scale(sa_at + static_cast<size_t>(at) * tokens), load_scale(sw_at + at));
-    };
-    float* scales = reinterpret_cast<float*>(shared + S::kScales);
-    constexpr int kGroup = COLS < 32 ? COLS : (COLS == 128 ? 16 : 32);
+    if (step >= 2 && !wait_warp(filled + 8 * half, (step / 2 - 1) & 1)) healthy = false;
+  } else if (warp == 2) {
+    // (slots as in the panel kernel; a token past the end takes the last one's scale, its sums are not stored)
     int step = 0;
-    auto add_block = [&](float2& factors, int b) {  // (two sets of factors that stay in their registers, as above)
-      const int half = step & 1;
-      // the products of the block's scales, for everybody: written to the half that was read two steps ago
-      if (fetches) scales[half * COLS + mine] = token < tokens ? __fmul_rn(factors.x, factors.y) : 0.0f;
-      factors = factors_at(b + 2);
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      // (no way out of the loop: the other warps count on this one at the barrier above)
-      if (healthy) healthy = wait_warp(filled + 8 * half, (step / 2) & 1);
-      fence_after_sync();
-      const float4* scale4 = reinterpret_cast<const float4*>(scales + half * COLS);
+    for (int tile = cluster; tile < tiles && healthy; tile += clusters) {
+      const int token0 = tile % token_tiles * COLS, visible = min(COLS, tokens - token0);
+      const float* tokens_at = sa + static_cast<size_t>(first) * tokens + token0;
+      const float* weight = sw + static_cast<size_t>(tile / token_tiles) * blocks + first;
+      for (int b = 0; b < count; ++b, ++step) {
+        const int s = step % kStages;
+        if (step >= kStages && !(healthy = wait_warp(empty + 8 * s, (step / kStages - 1) & 1))) break;
+        const uint32_t slot = base + S::kScales + (step % S::kSlots) * (S::kSlotFloats * 4);
 #pragma unroll
-      for (int g = 0; g < COLS / kGroup; ++g) {
-        uint32_t d[kGroup];
-        if constexpr (kGroup == 16) load16(lane_base + half * COLS + g * kGroup, d);
-        else load32(lane_base + half * COLS + g * kGroup, d);
-        wait_loads(d);
-        if (g + 1 == COLS / kGroup) {
-          fence_before_sync();
-          __syncwarp();
-          if (lane == 0) barrier_arrive(drained + 8 * half);
-        }
+        for (int i = 0; i < COLS; i += 32)
+          if (i + lane < COLS) copy_scale(slot + (i + lane) * 4, tokens_at + min(i + lane, visible - 1));
+        if (lane == 0) copy_scale(slot + COLS * 4, weight + b);
+        copies_arrive(full + 8 * s);
+        tokens_at += tokens;
+      }
+    }
+    copies_wait();
+  } else {
+    constexpr int kMine = S::kMine, kGroup = kMine < 32 ? kMine : 32, kAdding = S::kThreads - 128;
+    const int quarter = warp & 3, row = quarter * 32 + lane, col0 = ((warp - 4) >> 2) * kMine;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + col0;
+    const float* scales = reinterpret_cast<const float*>(shared + S::kScales);
+    float* partial = reinterpret_cast<float*>(shared + S::kPartial);
+    int step = 0, done = 0;
+    for (int tile = cluster; tile < tiles; tile += clusters, ++done) {
+      float sum[kMine];  // this thread's output row, this warp's tokens
 #pragma unroll
-        for (int i = 0; i < kGroup; i += 4) {
-          const float4 f = scale4[(g * kGroup + i) / 4];
-          float* to = sum + g * kGroup + i;
-          to[0] = fmaf(f.x, __uint_as_float(d[i]), to[0]);
-          to[1] = fmaf(f.y, __uint_as_float(d[i + 1]), to[1]);
-          to[2] = fmaf(f.z, __uint_as_float(d[i + 2]), to[2]);
-          to[3] = fmaf(f.w, __uint_as_float(d[i + 3]), to[3]);
+      for (int i = 0; i < kMine; ++i) sum[i] = 0.0f;
+      for (int b = 0; b < count; ++b, ++step) {
+        const int half = step & 1;
+        if (!(healthy = wait_warp(filled + 8 * half, (step / 2) & 1))) break;
+        fence_after_sync();
+        const float* slot = scales + (step % S::kSlots) * S::kSlotFloats;
+        const float2 weight = make_float2(slot[COLS], slot[COLS]);
+#pragma unroll
+        for (int g = 0; g < kMine; g += kGroup) {
+          uint32_t d[kGroup];
+          if constexpr (kGroup == 16) load16(lane_base + half * COLS + g, d);
+          else load32(lane_base + half * COLS + g, d);
+          float4 f[kGroup / 4];
+#pragma unroll
+          for (int i = 0; i < kGroup / 4; ++i) f[i] = reinterpret_cast<const float4*>(slot + col0 + g)[i];
+          wait_loads(d);
+          if (g + kGroup == kMine) {
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) barrier_arrive(drained + 8 * half);
+          }
+#pragma unroll
+          for (int i = 0; i < kGroup; i += 2) {
+            const float2 scale = mul2(i % 4 == 0 ? make_float2(f[i / 4].x, f[i / 4].y) : make_float2(f[i / 4].z, f[i / 4].w), weight);
+            const float2 r = fma2(scale, make_float2(__uint_as_float(d[i]), __uint_as_float(d[i + 1])),
+                                  make_float2(sum[g + i], sum[g + i + 1]));
+            sum[g + i] = r.x;
+            sum[g + i + 1] = r.y;
+          }
         }
       }
-      ++step;
-    };
-    float2 even = factors_at(0), odd = factors_at(1);
-    for (int b = 0; b < count; b += 2) {
-      add_block(even, b);
-      if (b + 1 < count) add_block(odd, b + 1);
+      if (!healthy) break;
+      // this CTA's sums, once the cluster has read the last tile's; then everybody's, added in rank order
+      if (done > 0 && !(healthy = wait_cluster(released, (done - 1) & 1))) break;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) partial[(col0 + i) * kRows + row] = sum[i];
+      __syncwarp();
+      if (lane < splits) arrive_at(ready, lane);
+      if (!(healthy = wait_cluster(ready, done & 1))) break;
+      const int row0 = tile / token_tiles * kRows, token0 = tile % token_tiles * COLS;
+      const int items = min(COLS, tokens - token0) * (kRows / 4);  // (token, four outputs)
+      for (int item = rank * kAdding + (threadIdx.x - 128); item < items; item += splits * kAdding) {
+        const int t = item / (kRows / 4), r = item % (kRows / 4) * 4;
+        const uint32_t at = base + S::kPartial + static_cast<uint32_t>((t * kRows + r) * 4);
+        float4 total = load_from(at, 0);
+        for (int from = 1; from < splits; ++from) {
+          const float4 p = load_from(at, from);
+          total = make_float4(total.x + p.x, total.y + p.y, total.z + p.z, total.w + p.w);
+        }
+        if (row0 + r < out_features)
+          *reinterpret_cast<uint2*>(out + static_cast<size_t>(token0 + t) * out_features + row0 + r) =
+              make_uint2(pack_bf16x2(total.x, total.y), pack_bf16x2(total.z, total.w));
+      }
+      __syncwarp();
+      if (lane < splits) arrive_at(released, lane);
     }
   }
   if (!healthy) atomicExch(&g_error, 1u);
   __syncwarp();
   fence_before_sync();
-  __syncthreads();  // every copy has landed and every product is complete: the stages are free
-  if (warp == 1)
+  __syncthreads();
+  if (warp == 2)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kColumns) : "memory");
-  float* partial = reinterpret_cast<float*>(shared);  // [token][output row]
-  if (warp >= 2) {
-#pragma unroll
-    for (int i = 0; i < COLS; ++i) partial[i * kRows + row] = sum[i];
-  }
-  // (all threads of all CTAs of the cluster come here, healthy or not)
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  // rank r finishes the items r, r + splits, ... of threads-many: item = (token, four outputs)
-  const int visible = min(COLS, tokens - token0);
-  for (int item = rank * kThreads + threadIdx.x; item < visible * (kRows / 4); item += splits * kThreads) {
-    const int t = item / (kRows / 4), r = (item % (kRows / 4)) * 4;
-    const uint32_t at = base + static_cast<uint32_t>((t * kRows + r) * 4);
-    float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int from = 0; from < splits; ++from) {
-      uint32_t there;
-      float4 p;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(from));
-      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                   : "=f"(p.x), "=f"(p.y), "=f"(p.z), "=f"(p.w)
-                   : "r"(there)
-                   : "memory");
-      total.x += p.x;
-      total.y += p.y;
-      total.z += p.z;
-      total.w += p.w;
-    }
-    if (row0 + r < out_features)
-      *reinterpret_cast<uint2*>(out + static_cast<size_t>(token0 + t) * out_features + row0 + r) =
-          make_uint2(pack_bf16x2(total.x, total.y), pack_bf16x2(total.z, total.w));
-  }
-  // no CTA leaves while another may still read its sums
   __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_sync();  // no CTA leaves while another may still read its sums or arrive on its barriers
 }
 
 }  // namespace strip
@@ -569,20 +607,33 @@ int launch_panel(const Problem& p) {
   return host::launch_status();
 }
 
-// CTAs that share a tile's blocks of K: the count with the least time on the busiest SM, in blocks, plus what joining
-// the sums costs (measured as about two blocks).
-int strip_splits(int tiles, int blocks, int slots) {
-  int best = 1;
-  double least = 1e300;
-  for (int s = 1; s <= strip::kMaxSplits && s <= blocks; ++s) {
-    const double waves = (static_cast<long long>(tiles) * s + slots - 1) / slots;
-    const double time = waves * ((blocks + s - 1) / s) + (s > 1 ? 2.0 : 0.0);
-    if (time < least) {
-      least = time;
-      best = s;
+// Clusters of `splits` CTAs that are resident at once (one CTA per SM; a cluster lives inside one group of SMs, so that
+// sizes that do not divide the groups leave SMs idle: 74 of two, 45 of three, 33 of four, 15 of seven or eight).
+template <auto kKernel, int kThreads>
+int resident_clusters(int splits, int shared) {
+  constexpr int kMaxDevices = 64;
+  static std::atomic<int> cache[kMaxDevices][strip::kMaxSplits + 1] = {};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMaxDevices) return 1;
+  int n = cache[device][splits].load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(splits);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = shared;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeClusterDimension;
+    attribute[0].val.clusterDim.x = splits;
+    attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
+    config.attrs = attribute;
+    config.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kKernel, &config) != cudaSuccess || n < 1) {
+      (void)cudaGetLastError();
+      n = 1;
     }
+    cache[device][splits].store(n, std::memory_order_relaxed);
   }
-  return best;
+  return n;
 }
 
 template <int COLS>
@@ -595,25 +646,38 @@ int launch_strip(const Problem& p) {
   if (!encode_map(&a, p.activations, p.tokens, p.in_features, COLS) ||
       !encode_map(&w, p.weights, p.out_features, p.in_features, strip::kRows))
     return host::kNotSupported;
-  const unsigned out_tiles = (p.out_features + strip::kRows - 1) / strip::kRows, token_tiles = (p.tokens + COLS - 1) / COLS;
-  if (out_tiles > 65535u || token_tiles > 65535u) return host::kNotSupported;
-  const int splits = strip_splits(static_cast<int>(out_tiles * token_tiles), p.blocks,
-                                  host::current_device_sm_count() * S::kCtasPerSm);
+  const int out_tiles = (p.out_features + strip::kRows - 1) / strip::kRows, token_tiles = (p.tokens + COLS - 1) / COLS;
+  if (static_cast<long long>(out_tiles) * token_tiles > 0x7fffffff / 2) return host::kNotSupported;
+  const int tiles = out_tiles * token_tiles;
+  // CTAs that share a tile's blocks of K: the count with the fewest blocks on the busiest CTA, joining the sums counted
+  // as kJoin blocks
+  constexpr double kJoin = 3.0;
+  int splits = 1, clusters = 1;
+  double least = 1e300;
+  for (int s = 1; s <= strip::kMaxSplits && s <= p.blocks; ++s) {
+    const int resident = resident_clusters<kernel, S::kThreads>(s, S::kShared);
+    const double time = static_cast<double>((tiles + resident - 1) / resident) * ((p.blocks + s - 1) / s) + (s > 1 ? kJoin : 0.0);
+    if (time < least) {
+      least = time;
+      splits = s;
+      clusters = tiles < resident ? tiles : resident;
+    }
+  }
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(splits, out_tiles, token_tiles);
-  config.blockDim = dim3(strip::kThreads);
+  config.gridDim = dim3(clusters * splits);
+  config.blockDim = dim3(S::kThreads);
   config.dynamicSmemBytes = S::kShared;
   config.stream = p.stream;
   cudaLaunchAttribute attributes[2];
   attributes[0].id = cudaLaunchAttributeClusterDimension;
   attributes[0].val.clusterDim.x = splits;
-  attributes[0].val.clusterDim.y = 1;
-  attributes[0].val.clusterDim.z = 1;
+  attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
   attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attributes[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attributes;
   config.numAttrs = host::overlap_allowed() ? 2 : 1;
-  (void)cudaLaunchKernelEx(&config, kernel, a, w, p.activation_scales, p.weight_scales, p.tokens, p.out_features, p.blocks, p.out);
+  (void)cudaLaunchKernelEx(&config, kernel, a, w, p.activation_scales, p.weight_scales, p.tokens, p.out_features, p.blocks,
+                           token_tiles, tiles, splits, p.out);
   return host::launch_status();
 }
 

@@ -150,17 +150,7 @@ __device__ __forceinline__ void load_box(uint32_t shared_address, const void* ma
                "l"(map), "r"(x), "r"(y), "r"(barrier)
                : "memory");
 }
-__device__ __forceinline__ void store_box(const void* map, int x, int y, uint32_t shared_address) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
-               "r"(shared_address)
-               : "memory");
-}
-__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-// all but the newest N stores have read their shared memory / have completed
-template <int N>
-__device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
-template <int N>
-__device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void prefetch_map(const void* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
 // wait_loads() that also names the registers waited for, so that no use of them can be scheduled in front of it
 __device__ __forceinline__ void wait_loads(uint32_t (&r)[32]) {

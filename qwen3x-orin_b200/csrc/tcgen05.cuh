@@ -91,8 +91,8 @@ __device__ __forceinline__ uint64_t operand_descriptor_mn(uint32_t shared_addres
 constexpr uint32_t kBOperandMnMajor = 1u << 16;  // or-ed into an instruction descriptor
 
 // ---- E4M3 x E4M3 -> FP32 (32 elements of k per instruction; rows of 128 codes are the same 128 bytes as 64 bf16)
-__host__ __device__ constexpr uint32_t instruction_descriptor_e4m3(int n) {
-  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
+__host__ __device__ constexpr uint32_t instruction_descriptor_e4m3(int n, int m = 128) {
+  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 __device__ __forceinline__ void mma_e4m3(uint32_t accumulator, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -101,6 +101,19 @@ __device__ __forceinline__ void mma_e4m3(uint32_t accumulator, uint64_t a, uint6
       : "memory");
 }
 
+// The same on a pair of CTAs: M = 256, each CTA holds 128 rows of A and of the accumulator and n / 2 rows of B, at the
+// same offsets; the leader (the even rank of the two) issues, and a commit arrives on both CTAs' copies of the barrier.
+__device__ __forceinline__ void mma_e4m3_pair(uint32_t accumulator, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(accumulator),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint32_t barrier, int leader) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(barrier),
+               "h"(static_cast<uint16_t>(3 << leader))
+               : "memory");
+}
 // One lane of a converged warp, always the same one.  A warp that issues walks its loop with all lanes and lets this one
 // issue: addresses and descriptors then stay warp-uniform, which is what the tensor instructions take (a loop entered by
 // one lane alone moves every one of them into uniform registers again, a hundred cycles per instruction).
@@ -150,6 +163,24 @@ __device__ __forceinline__ void load_box(uint32_t shared_address, const void* ma
                "l"(map), "r"(x), "r"(y), "r"(barrier)
                : "memory");
 }
+// The same into this CTA of a pair, completing on a barrier of either CTA of it (a cluster address).
+__device__ __forceinline__ void load_box_pair(uint32_t shared_address, const void* map, int x, int y, uint32_t barrier) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                   shared_address),
+               "l"(map), "r"(x), "r"(y), "r"(barrier)
+               : "memory");
+}
+__device__ __forceinline__ void store_box(const void* map, int x, int y, uint32_t shared_address) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
+               "r"(shared_address)
+               : "memory");
+}
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// all but the newest N stores have read their shared memory / have completed
+template <int N>
+__device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+template <int N>
+__device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void prefetch_map(const void* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
 // wait_loads() that also names the registers waited for, so that no use of them can be scheduled in front of it

@@ -38,12 +38,9 @@ __device__ __forceinline__ void block_product(uint32_t accumulator, uint32_t a, 
     mma_e4m3(accumulator, operand_descriptor(a + step * 32), operand_descriptor(b + step * 32), idesc, step > 0 ? 1u : 0u);
 }
 
-// The cluster: a barrier of all its threads, an arrival on a rank's copy of a barrier, a rank's copy of four floats, and the
-// bounded wait for arrivals from other CTAs.
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// The same in two parts, without publishing memory (barriers are published by their own fence).
+// The cluster: a barrier of all its threads in two parts, a rank's copy of an address, and an arrival on a rank's copy of a
+// barrier.  They do not publish memory to the cluster, which would cost a fence of a thousand cycles: they hand on barriers
+// and tensor memory, which have fences of their own, or say that values have been read.
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t at_rank(uint32_t address, int rank) {
@@ -51,30 +48,17 @@ __device__ __forceinline__ uint32_t at_rank(uint32_t address, int rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(address), "r"(rank));
   return there;
 }
-__device__ __forceinline__ void arrive_cluster(uint32_t there) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(there) : "memory");
-}
-// The same without publishing memory to the cluster, which costs a fence of a thousand cycles: for arrivals that hand on
-// tensor memory, whose accesses have fences of their own.
 __device__ __forceinline__ void arrive_remote(uint32_t there) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(there) : "memory");
 }
-// A float into another CTA's shared memory; completes its four bytes on a barrier of that CTA.
-__device__ __forceinline__ void push(uint32_t there, float value, uint32_t barrier_there) {
-  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(there), "f"(value),
-               "r"(barrier_there)
+// Four floats into another CTA's shared memory; their bytes complete on a barrier of that CTA.
+__device__ __forceinline__ void push(uint32_t there, const float4& v, uint32_t barrier_there) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(there), "f"(v.x),
+               "f"(v.y), "f"(v.z), "f"(v.w), "r"(barrier_there)
                : "memory");
 }
 __device__ __forceinline__ float4 add4(const float4& a, const float4& b) {
   return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
-}
-__device__ __forceinline__ float4 load_from(uint32_t address, int rank) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(at_rank(address, rank))
-               : "memory");
-  return v;
 }
 // One FP32 from global to shared memory; the lane's copies so far arrive on the barrier, which counts on that arrival,
 // when they have landed; and the wait for them at the end.
@@ -94,11 +78,6 @@ __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;
 __device__ __forceinline__ bool wait_warp(uint32_t barrier, uint32_t parity) {
   return __all_sync(kFullMask, barrier_try(barrier, parity)) || __all_sync(kFullMask, wait_bounded(barrier, parity));
 }
-__device__ __forceinline__ bool wait_cluster(uint32_t barrier, uint32_t parity) {
-  const bool done = wait_warp(barrier, parity);
-  asm volatile("fence.acq_rel.cluster;" ::: "memory");
-  return done;
-}
 __device__ __forceinline__ void block_product_pair(uint32_t accumulator, uint32_t a, uint32_t b, uint32_t idesc) {
 #pragma unroll
   for (int step = 0; step < kBlockK / 32; ++step)
@@ -110,47 +89,36 @@ __device__ __forceinline__ uint32_t shared_address(const void* p) { return stati
 // ------------------------------------------------------------------------------------------------------------- panel
 namespace panel {
 
+// Tiles of 128 tokens x 128 outputs, one CTA each: for products with too few tiles of 256 x 256 to give every pair of SMs
+// one.
 constexpr int kRows = 128;                  // tokens of a tile
+constexpr int kCols = 128;                  // outputs of a tile
 constexpr int kThreads = 384;               // warp 0 fetches codes, 2 scales, 1 and 3 issue, 4 to 11 add up
-constexpr int kAdders = 8;                  // warps: 4 lane quarters x 2 column halves
+constexpr int kAdders = 8;                  // warps: 4 lane quarters x 2 halves of the outputs
+constexpr int kMine = kCols / 2;            // outputs of one adding warp
 constexpr int kLaunchRegisters = 168;       // 65536 / 384, rounded down to 8
-constexpr int kSlotFloats = kRows + 4;
 constexpr int kBand = 16;                   // token tiles walked together
+constexpr int kBuffers = 4;                 // accumulators, one block of K after the other
+constexpr int kStageBytes = (kRows + kCols) * kRowBytes;
+constexpr int kStages = 6;
+constexpr int kSlots = 16;                  // of scales, one per block in flight
+constexpr int kSlotFloats = kRows + 4;      // the tokens', the weight block's, 3 unused
+constexpr int kStore = kStages * kStageBytes;                  // [adder][32 rows][32 outputs] bf16
+constexpr int kScales = kStore + kAdders * 32 * 64;
+constexpr int kBarriers = kScales + kSlots * kSlotFloats * 4;
+constexpr int kTmemSlot = kBarriers + 8 * (2 * kStages + 2 * kBuffers);
+constexpr int kShared = kTmemSlot + 16;
+static_assert(kStages + kBuffers <= kSlots, "see the warp that fetches scales");
+static_assert(kShared <= 232448, "shared memory of one CTA");
 
-// Four accumulators of 128 columns.  256 outputs: one for each half of the outputs and parity of the block of K, each half
-// added up by four warps; 128 outputs: one for each block of K modulo four, half of its columns for four warps.
-constexpr int kBuffers = 4, kBufferCols = 128;
-
-template <int COLS>
-struct Shape {
-  static constexpr int kHalves = COLS / kBufferCols;              // products per block
-  static constexpr int kMine = COLS / 2;                          // outputs of one adding warp
-  static constexpr int kReaders = kAdders / kHalves;              // warps that read one accumulator
-  static constexpr int kTurn = kBuffers / kHalves;                // blocks until an accumulator comes round again
-  static constexpr int kStageBytes = (kRows + COLS) * kRowBytes;
-  static constexpr int kStages = COLS == 256 ? 4 : 6;
-  static constexpr int kSlots = COLS == 256 ? 8 : 16;             // of scales, one per block in flight
-  static constexpr int kStore = kStages * kStageBytes;          // [adder][32 rows][32 outputs] bf16
-  static constexpr int kScales = kStore + kAdders * 32 * 64;    // [slot][128 tokens, 2 column halves, 2 unused] FP32
-  static constexpr int kBarriers = kScales + kSlots * kSlotFloats * 4;
-  static constexpr int kShared = 1024 + kBarriers + 256;  // (1024: the stages start on a 1024-byte boundary)
-  static_assert(kStages + kTurn <= kSlots, "see the warp that fetches scales");
-  static_assert(16 * kStages + 16 * kBuffers + 4 <= 256 && kShared <= 232448, "shared memory of one CTA");
-};
-
-template <int COLS>
 __global__ void __launch_bounds__(kThreads, 1)
     block_gemm_panel_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                             const float* __restrict__ sa, const float* __restrict__ sw, int tokens, int out_features,
                             int blocks, int row_tiles, int col_tiles, uint16_t* __restrict__ out) {
-  using S = Shape<COLS>;
-  constexpr int kStages = S::kStages;
-  extern __shared__ uint8_t raw[];
-  uint8_t* shared = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  extern __shared__ __align__(1024) uint8_t shared[];
   const uint32_t base = shared_address(shared);
-  const uint32_t full = base + S::kBarriers, empty = full + 8 * kStages, filled = empty + 8 * kStages,
-                 drained = filled + 8 * kBuffers;
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(shared + S::kBarriers + 16 * kStages + 16 * kBuffers);
+  const uint32_t full = base + kBarriers, empty = full + 8 * kStages, filled = empty + 8 * kStages, drained = filled + 8 * kBuffers;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(shared + kTmemSlot);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles = row_tiles * col_tiles;
 
@@ -159,17 +127,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_map(&map_w);
     for (int s = 0; s < kStages; ++s) {
       barrier_init(full + 8 * s, 1 + 32);  // the codes' fetcher and every lane of the scales'
-      barrier_init(empty + 8 * s, S::kHalves);
+      barrier_init(empty + 8 * s, 1);
     }
     for (int i = 0; i < kBuffers; ++i) {
       barrier_init(filled + 8 * i, 1);
-      barrier_init(drained + 8 * i, S::kReaders);
+      barrier_init(drained + 8 * i, kAdders);
     }
     barrier_init_fence();
   }
   if (warp == 2) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(const_cast<uint32_t*>(tmem_slot))),
-                 "r"(kBuffers * kBufferCols)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + kTmemSlot), "r"(kBuffers * kCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -201,11 +168,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int b = 0; b < blocks; ++b, ++step) {
           const int s = step % kStages;
           if (step >= kStages && !(healthy = wait_warp(empty + 8 * s, (step / kStages - 1) & 1))) break;
-          const uint32_t at = base + s * S::kStageBytes;
+          const uint32_t at = base + s * kStageBytes;
           if (elect_one()) {
-            barrier_expect(full + 8 * s, S::kStageBytes);
+            barrier_expect(full + 8 * s, kStageBytes);
             load_box(at, &map_a, b * kBlockK, row_tile * kRows, full + 8 * s);
-            load_box(at + kRows * kRowBytes, &map_w, b * kBlockK, col_tile * COLS, full + 8 * s);
+            load_box(at + kRows * kRowBytes, &map_w, b * kBlockK, col_tile * kCols, full + 8 * s);
           }
         }
       }
@@ -215,66 +182,64 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 2) {
       // The scales of a block, copied without passing through registers (a load held in one for two blocks was measured to
       // hold up the whole warp wherever the compiler moved it).  A slot is free again: when step
-      // t - kStages has left its stage, its accumulator had come round, so step t - kStages - kTurn was drained, its scales
+      // t - kStages has left its stage, its accumulator had come round, so step t - kStages - kBuffers was drained, its scales
       // and all older ones read; slot t % kSlots holds a step at least that old.
-      const int weight_rows = (out_features + kBlockK - 1) / kBlockK;
       int step = 0;
       for (int tile = blockIdx.x; tile < tiles && healthy; tile += gridDim.x) {
         int row_tile, col_tile;
         tile_at(tile, row_tile, col_tile);
         const float* rows = sa + row_tile * kRows;
         const int visible = min(kRows, tokens - row_tile * kRows);
-        // (a weight block past the end reads the last one's scale: its sums are not stored)
-        const int weight_row = min((col_tile * COLS + (lane & 1) * (COLS / 2)) / kBlockK, weight_rows - 1);
-        const float* weight = sw + static_cast<size_t>(weight_row) * blocks;
+        const float* weight = sw + static_cast<size_t>(col_tile) * blocks;
         for (int b = 0; b < blocks; ++b, ++step) {
           const int s = step % kStages;
           if (step >= kStages && !(healthy = wait_warp(empty + 8 * s, (step / kStages - 1) & 1))) break;
-          const uint32_t slot = base + S::kScales + (step % S::kSlots) * kSlotFloats * 4;
+          const uint32_t slot = base + kScales + (step % kSlots) * kSlotFloats * 4;
 #pragma unroll
           for (int i = 0; i < kRows; i += 32) copy_scale(slot + (i + lane) * 4, rows + min(i + lane, visible - 1));
-          if (lane < 2) copy_scale(slot + (kRows + lane) * 4, weight + b);
+          if (lane == 0) copy_scale(slot + kRows * 4, weight + b);
           copies_arrive(full + 8 * s);
           rows += tokens;
         }
       }
       copies_wait();
     } else {
-      // Two warps issue in turn: the halves of the outputs, or the even and the odd blocks.  A warp's instructions wait in
-      // line behind its own products, so one warp alone would test the next barriers only once its products are in the
-      // pipe, and the pipe would run dry for the time of those tests (measured: 900 cycles per block instead of 512).
-      const int turn = warp >> 1, steps = (tiles - static_cast<int>(blockIdx.x) + gridDim.x - 1) / gridDim.x * blocks;
-      int step = S::kHalves == 2 ? 0 : turn, last = -1;
-      for (; step < steps; step += S::kHalves == 2 ? 1 : 2) {
-        const int s = step % kStages, round = step / S::kTurn;
-        const int buffer = S::kHalves == 2 ? (step & 1) * 2 + turn : step % kBuffers;
+      // Warp 1 issues the even steps, warp 3 the odd ones.  A warp's instructions wait in line behind its own products, so
+      // one warp alone would test the next barriers only once its products are in the pipe, and the pipe would run dry
+      // for the time of those tests.
+      const int steps = (tiles - static_cast<int>(blockIdx.x) + gridDim.x - 1) / gridDim.x * blocks;
+      int step = warp >> 1;
+      for (; step < steps; step += 2) {
+        const int s = step % kStages, buffer = step % kBuffers, round = step / kBuffers;
         if (!(healthy = wait_warp(full + 8 * s, (step / kStages) & 1))) break;
         if (round > 0 && !(healthy = wait_warp(drained + 8 * buffer, (round - 1) & 1))) break;
         fence_after_sync();
-        const uint32_t at = base + s * S::kStageBytes;
+        const uint32_t at = base + s * kStageBytes;
         if (elect_one()) {
-          block_product(tmem + buffer * kBufferCols, at, at + kRows * kRowBytes + (S::kHalves == 2 ? turn * kBufferCols * kRowBytes : 0),
-                        instruction_descriptor_e4m3(kBufferCols));
-          commit(empty + 8 * s);
+          block_product(tmem + buffer * kCols, at, at + kRows * kRowBytes, instruction_descriptor_e4m3(kCols));
           commit(filled + 8 * buffer);
+          commit(empty + 8 * s);
         }
         __syncwarp();
-        last = step;
       }
-      // (products complete in order: after this warp's last one none of them is reading shared memory)
-      if (last >= 0) {
-        const int buffer = S::kHalves == 2 ? (last & 1) * 2 + turn : last % kBuffers;
-        if (!wait_warp(filled + 8 * buffer, (last / S::kTurn) & 1)) healthy = false;
+      // An empty commit where the next product would arrive, and no sooner: the adding warps ask about it after the last
+      // block, and a question about products that never come would hold them for microseconds.  It is complete when all
+      // products of this warp are, so that none of them reads shared memory any more.
+      if (healthy && step >= kBuffers) healthy = wait_warp(drained + 8 * (step % kBuffers), (step / kBuffers - 1) & 1);
+      if (healthy) {
+        if (elect_one()) commit(filled + 8 * (step % kBuffers));
+        __syncwarp();
+        healthy = wait_warp(filled + 8 * (step % kBuffers), (step / kBuffers) & 1);
+      } else if (step >= 2) {
+        wait_warp(filled + 8 * ((step - 2) % kBuffers), ((step - 2) / kBuffers) & 1);
       }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-    constexpr int kMine = S::kMine, kTurn = S::kTurn;
     const int quarter = warp & 3, half_cols = (warp - 4) >> 2;
-    const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (S::kHalves == 2 ? 0 : half_cols * kMine);
-    auto buffer_of = [&](int at) { return S::kHalves == 2 ? (at & 1) * 2 + half_cols : at % kBuffers; };
-    uint8_t* store = shared + S::kStore + (warp - 4) * 32 * 64;
-    const uint32_t row_scale = base + S::kScales + (quarter * 32 + lane) * 4, col_scale = base + S::kScales + (kRows + half_cols) * 4;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half_cols * kMine;
+    uint8_t* store = shared + kStore + (warp - 4) * 32 * 64;
+    const uint32_t row_scale = base + kScales + (quarter * 32 + lane) * 4, col_scale = base + kScales + kRows * 4;
     int step = 0;
     for (int tile = blockIdx.x; tile < tiles && healthy; tile += gridDim.x) {
       float sum[kMine];
@@ -287,17 +252,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       float2 factors;
       auto begin = [&](int at) {  // a block whose products are complete
         fence_after_sync();
-        load32(lane_base + buffer_of(at) * kBufferCols, d[0]);
-        factors = make_float2(load_shared(row_scale + at % S::kSlots * (kSlotFloats * 4)),
-                              load_shared(col_scale + at % S::kSlots * (kSlotFloats * 4)));
+        load32(lane_base + at % kBuffers * kCols, d[0]);
+        factors = make_float2(load_shared(row_scale + at % kSlots * (kSlotFloats * 4)),
+                              load_shared(col_scale + at % kSlots * (kSlotFloats * 4)));
       };
       bool begun = false;
       for (int b = 0; b < blocks; ++b) {
         if (!begun) {
-          if (!(healthy = wait_warp(filled + 8 * buffer_of(step), (step / kTurn) & 1))) break;
+          if (!(healthy = wait_warp(filled + 8 * (step % kBuffers), (step / kBuffers) & 1))) break;
           begin(step);
         }
-        const uint32_t columns = lane_base + buffer_of(step) * kBufferCols;
+        const uint32_t columns = lane_base + step % kBuffers * kCols;
         const float scale = __fmul_rn(factors.x, factors.y);
         bool complete = false;
 #pragma unroll
@@ -305,11 +270,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           wait_loads(d[g & 1]);
           if (g + 1 < kMine / 32) {
             load32(columns + (g + 1) * 32, d[(g + 1) & 1]);
-            if (g + 2 == kMine / 32) complete = barrier_try(filled + 8 * buffer_of(step + 1), ((step + 1) / kTurn) & 1);
+            if (g + 2 == kMine / 32) complete = barrier_try(filled + 8 * ((step + 1) % kBuffers), ((step + 1) / kBuffers) & 1);
           } else {
             fence_before_sync();
             __syncwarp();
-            if (lane == 0) barrier_arrive(drained + 8 * buffer_of(step));
+            if (lane == 0) barrier_arrive(drained + 8 * (step % kBuffers));
             ++step;
             begun = b + 1 < blocks && __all_sync(kFullMask, complete);
             if (begun) begin(step);
@@ -327,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!healthy) break;
       int row_tile, col_tile;
       tile_at(tile, row_tile, col_tile);
-      const int row0 = row_tile * kRows + quarter * 32, col0 = col_tile * COLS + half_cols * kMine;
+      const int row0 = row_tile * kRows + quarter * 32, col0 = col_tile * kCols + half_cols * kMine;
       // 32 rows x 32 outputs at a time through the warp's own 2 KB, so that a store covers whole 64-byte pieces of eight
       // rows (16-byte parts permuted by the row: free of bank conflicts both ways)
 #pragma unroll
@@ -356,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_before_sync();
   __syncthreads();
   if (warp == 2)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kBuffers * kBufferCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kBuffers * kCols) : "memory");
 }
 
 }  // namespace panel
@@ -369,10 +334,6 @@ namespace pair {
 // fetches 32 KB instead of 48 KB per block of K, and an instruction of 128 columns reads 6 KB of shared memory instead
 // of 8 in its 64 cycles, which is what lets the accumulators be four of 128 columns: each half of the outputs has two, and
 // a half is read while three other products run.
-//
-// Few tiles leave SMs idle, so with kSplit a cluster of `splits` pairs shares the blocks of K of a tile: each pair adds up
-// its share, and the pairs exchange their FP32 sums through the staging area, one half of the outputs after the other:
-// everybody's warps of that half write, everybody adds the rows whose index is its pair's modulo `splits`, in pair order.
 constexpr int kRows = 128;                  // tokens of a CTA
 constexpr int kCols = 256;                  // outputs of a tile
 constexpr int kHalf = 128;                  // outputs of one product
@@ -388,77 +349,22 @@ constexpr int kSlotFloats = kRows + 4;      // the tokens', the two halves' weig
 constexpr int kStore = kStages * kStageBytes;                  // [adder][2][32 rows][64 outputs] bf16
 constexpr int kScales = kStore + kAdders * 2 * 32 * 128;
 constexpr int kBarriers = kScales + kSlots * kSlotFloats * 4;
-constexpr int kTmemSlot = kBarriers + 8 * (2 * kStages + 2 * kBuffers + 2 * kSlots + 2);
-constexpr int kMaxSplits = 4;
-static_assert(kScales - kStore == kRows * kHalf * 4, "the staging area holds one half's FP32 sums");
+constexpr int kTmemSlot = kBarriers + 8 * (2 * kStages + 2 * kBuffers + 2 * kSlots);
 constexpr int kShared = kTmemSlot + 16;
 static_assert(kShared <= 232448, "shared memory of one CTA");
 
-// The exchange of kSplit.  A row of a half is 512 bytes, its 16-byte pieces permuted by the row: a warp writes 32 rows of
-// one column and reads one row without bank conflicts.
-template <typename Store>
-__device__ __forceinline__ bool join_halves(const float (&sum)[kHalf], int half, int quarter, int adder, int lane, int rank,
-                                            int share, int splits, int& rounds, uint8_t* staging, uint32_t staging_at,
-                                            uint32_t ready, uint32_t released, Store&& store) {
-  for (int h = 0; h < 2; ++h, ++rounds) {
-    if (half == h) {
-      if (rounds > 0 && !wait_cluster(released, (rounds - 1) & 1)) return false;
-      const int row = quarter * 32 + lane;
-#pragma unroll
-      for (int piece = 0; piece < kHalf / 4; ++piece)
-        *reinterpret_cast<float4*>(staging + row * (kHalf * 4) + ((piece ^ (row & 31)) << 4)) =
-            make_float4(sum[piece * 4], sum[piece * 4 + 1], sum[piece * 4 + 2], sum[piece * 4 + 3]);
-      __syncwarp();
-      if (lane < splits) arrive_cluster(at_rank(ready, lane * 2 + rank));
-    }
-    if (!wait_cluster(ready, rounds & 1)) return false;
-    // four rows' loads are in flight together: one after the other they took 7 us per half
-    constexpr int kBatch = 4;
-    for (int row0 = share + adder * splits; row0 < kRows; row0 += kBatch * kAdders * splits) {
-      float4 p[kBatch][kMaxSplits];
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int row = row0 + i * kAdders * splits;
-        const uint32_t at = staging_at + row * (kHalf * 4) + ((lane ^ (row & 31)) << 4);
-#pragma unroll
-        for (int from = 0; from < kMaxSplits; ++from)
-          p[i][from] = from < splits && row < kRows ? load_from(at, from * 2 + rank) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      }
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        float4 total = p[i][0];
-#pragma unroll
-        for (int from = 1; from < kMaxSplits; ++from)
-          if (from < splits) total = add4(total, p[i][from]);
-        if (row0 + i * kAdders * splits < kRows) store(row0 + i * kAdders * splits, h * kHalf + lane * 4, total);
-      }
-    }
-    __syncwarp();
-    if (lane < splits) arrive_cluster(at_rank(released, lane * 2 + rank));
-  }
-  return true;
-}
-
-template <bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
     block_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                            const __grid_constant__ CUtensorMap map_out, const float* __restrict__ sa,
                            const float* __restrict__ sw, int tokens, int out_features, int blocks, int row_tiles,
-                           int col_tiles, int splits, uint16_t* __restrict__ out) {
+                           int col_tiles) {
   extern __shared__ __align__(1024) uint8_t shared[];
   const uint32_t base = shared_address(shared);
   const uint32_t full = base + kBarriers, empty = full + 8 * kStages, filled = empty + 8 * kStages,
-                 drained = filled + 8 * kBuffers, scaled = drained + 8 * kBuffers, taken = scaled + 8 * kSlots,
-                 ready = taken + 8 * kSlots, released = ready + 8;
+                 drained = filled + 8 * kBuffers, scaled = drained + 8 * kBuffers, taken = scaled + 8 * kSlots;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(shared + kTmemSlot);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = blockIdx.x & 1, tiles = row_tiles * col_tiles;
-  const int share = kSplit ? (blockIdx.x >> 1) % splits : 0;  // of the blocks of K; the pair's place in the cluster
-  const int leader = share * 2;                               // the cluster rank of the pair's leader
-  const int cluster = kSplit ? (blockIdx.x >> 1) / splits : blockIdx.x >> 1;
-  const int clusters = kSplit ? (gridDim.x >> 1) / splits : gridDim.x >> 1;
-  const int first = kSplit ? static_cast<int>(static_cast<long long>(blocks) * share / splits) : 0;
-  const int count = kSplit ? static_cast<int>(static_cast<long long>(blocks) * (share + 1) / splits) - first : blocks;
+  const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, tiles = row_tiles * col_tiles;
 
   if (threadIdx.x == 0) {
     prefetch_map(&map_a);
@@ -476,10 +382,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       barrier_init(scaled + 8 * i, 32);
       barrier_init(taken + 8 * i, kAdders);
     }
-    if (kSplit) {
-      barrier_init(ready, kAdders / 2 * splits);
-      barrier_init(released, kAdders * splits);
-    }
     barrier_init_fence();
   }
   if (warp == 2) {
@@ -489,7 +391,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   fence_before_sync();
   __syncthreads();
-  cluster_sync();
+  cluster_arrive();
+  cluster_wait();
   fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   // only now: a successor that took this SM's tensor memory first would wait for this kernel and this kernel for it
@@ -509,13 +412,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 0) {
-      const uint32_t leader_full = at_rank(full, leader);
+      const uint32_t leader_full = at_rank(full, 0);
       int step = 0;
-      for (int tile = cluster; tile < tiles && healthy; tile += clusters) {
+      for (int tile = pair; tile < tiles && healthy; tile += pairs) {
         int row_tile, col_tile;
         tile_at(tile, row_tile, col_tile);
         const int row0 = (row_tile * 2 + rank) * kRows, col0 = col_tile * kCols + rank * (kHalf / 2);
-        for (int b = first; b < first + count; ++b, ++step) {
+        for (int b = 0; b < blocks; ++b, ++step) {
           const int s = step % kStages;
           if (step >= kStages && !(healthy = wait_warp(empty + 8 * s, (step / kStages - 1) & 1))) break;
           const uint32_t at = base + s * kStageBytes;
@@ -537,13 +440,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       // hold up the whole warp wherever the compiler moved it).
       const int weight_rows = (out_features + kBlockK - 1) / kBlockK;
       int step = 0;
-      for (int tile = cluster; tile < tiles && healthy; tile += clusters) {
+      for (int tile = pair; tile < tiles && healthy; tile += pairs) {
         int row_tile, col_tile;
         tile_at(tile, row_tile, col_tile);
         // (a token or weight block past the end takes the last one's scale: its sums are not stored)
         const int row0 = (row_tile * 2 + rank) * kRows;
         const float* weight = sw + static_cast<size_t>(min(col_tile * 2 + (lane & 1), weight_rows - 1)) * blocks;
-        for (int b = first; b < first + count; ++b, ++step) {
+        for (int b = 0; b < blocks; ++b, ++step) {
           const int slot = step % kSlots;
           if (step >= kSlots && !(healthy = wait_warp(taken + 8 * slot, (step / kSlots - 1) & 1))) break;
           const uint32_t at = base + kScales + slot * (kSlotFloats * 4);
@@ -554,14 +457,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           copies_arrive(scaled + 8 * slot);
         }
       }
+      // (the arrival without copies that the adding warps ask about after the last block)
+      if (healthy && step >= kSlots) healthy = wait_warp(taken + 8 * (step % kSlots), (step / kSlots - 1) & 1);
+      if (healthy) copies_arrive(scaled + 8 * (step % kSlots));
       copies_wait();
-    } else if (rank == 0) {
-      // Two warps issue, one for each half of the outputs.  A warp's instructions wait in line behind its own products, so
+    } else {
+      // Two warps of the leader issue, one for each half of the outputs.  A warp's instructions wait in line behind its own products, so
       // one warp alone would test the next barriers only once its products are in the pipe, and the pipe would run dry
       // for the time of those tests.
-      const int half = warp >> 1, steps = (tiles - cluster + clusters - 1) / clusters * count;
+      const int half = warp >> 1, steps = (tiles - pair + pairs - 1) / pairs * blocks;
       int step = 0;
-      for (; step < steps; ++step) {
+      for (; rank == 0 && step < steps; ++step) {
         const int s = step % kStages, buffer = (step & 1) * 2 + half;
         if (!(healthy = wait_warp(full + 8 * s, (step / kStages) & 1))) break;
         if (step >= 2 && !(healthy = wait_warp(drained + 8 * buffer, (step / 2 - 1) & 1))) break;
@@ -570,30 +476,41 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (elect_one()) {
           block_product_pair(tmem + buffer * kHalf, at, at + (kRows + half * (kHalf / 2)) * kRowBytes,
                              instruction_descriptor_e4m3(kHalf, 256));
-          commit_pair(filled + 8 * buffer, leader);
-          commit_pair(empty + 8 * s, leader);
+          commit_pair(filled + 8 * buffer);
+          commit_pair(empty + 8 * s);
         }
         __syncwarp();
       }
-      // (products complete in order: after this warp's last one none of them is reading shared memory)
-      if (step > 0 && !wait_warp(filled + 8 * (((step - 1) & 1) * 2 + half), ((step - 1) / 2) & 1)) healthy = false;
+      // The empty commit; it is complete when all products of this warp are, so that none of them reads shared memory any
+      // more, and both CTAs see it arrive before they end.
+      // (No sooner than a product could come: one that overtook a warp still waiting for the block before would turn the
+      // barrier's phase over twice.)
+      const int buffer = (steps & 1) * 2 + half;
+      if (rank == 0 && healthy && steps >= 2) healthy = wait_warp(drained + 8 * buffer, (steps / 2 - 1) & 1);
+      if (rank == 0 && healthy && elect_one()) commit_pair(filled + 8 * buffer);
+      __syncwarp();
+      if (healthy) healthy = wait_warp(filled + 8 * buffer, (steps / 2) & 1);
+      else if (step > 0) wait_warp(filled + 8 * (((step - 1) & 1) * 2 + half), ((step - 1) / 2) & 1);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * kHalf;
-    const uint32_t leader_drained = at_rank(drained, leader) + 8 * half;
+    const uint32_t leader_drained = at_rank(drained, 0) + 8 * half;
     const uint32_t row_scale = base + kScales + (quarter * 32 + lane) * 4, col_scale = base + kScales + (kRows + half) * 4;
     uint8_t* store = shared + kStore + (warp - 4) * 2 * 32 * 128;
     const uint32_t mine = filled + 8 * half;
-    int step = 0, rounds = 0;
-    for (int tile = cluster; tile < tiles && healthy; tile += clusters) {
+    int step = 0;
+    for (int tile = pair; tile < tiles && healthy; tile += pairs) {
       float sum[kHalf];
 #pragma unroll
       for (int i = 0; i < kHalf; ++i) sum[i] = 0.0f;
       // One block: 32 columns of its accumulator at a time, times its scales, onto the sums; the next 32 columns, which may
       // be the next block's first, are on their way meanwhile.  Whether that block's products are complete is asked
-      // before the last columns but one are added and answered after.
+      // before the last columns but one are added and answered after.  (After the very last block the
+      // answer comes from an empty commit and an arrival without copies: a question about products that never come would
+      // hold the warp for microseconds, and asking only before other blocks, by a branch or by another barrier, was
+      // measured to cost a tenth of the kernel.)
       uint32_t d[2][32];
       float2 factors;
       auto begin = [&](int at) {  // a block whose products and scales are there
@@ -603,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                               load_shared(col_scale + at % kSlots * (kSlotFloats * 4)));
       };
       bool begun = false;
-      for (int b = 0; b < count; ++b) {
+      for (int b = 0; b < blocks; ++b) {
         if (!begun) {
           if (!(healthy = wait_warp(mine + 16 * (step & 1), (step / 2) & 1) &&
                           wait_warp(scaled + 8 * (step % kSlots), (step / kSlots) & 1)))
@@ -618,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           wait_loads(d[g & 1]);
           if (g + 1 < kHalf / 32) {
             load32(columns + (g + 1) * 32, d[(g + 1) & 1]);
-            if (g + 2 == kHalf / 32) {  // (both asked, without a branch: the warp stays together)
+            if (g + 2 == kHalf / 32) {
               const bool products = barrier_try(mine + 16 * (~step & 1), ((step + 1) / 2) & 1);
               const bool scales = barrier_try(scaled + 8 * ((step + 1) % kSlots), ((step + 1) / kSlots) & 1);
               complete = products & scales;
@@ -631,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               barrier_arrive(taken + 8 * (step % kSlots));
             }
             ++step;
-            begun = b + 1 < count && __all_sync(kFullMask, complete);
+            begun = b + 1 < blocks && __all_sync(kFullMask, complete);
             if (begun) begin(step);
           }
 #pragma unroll
@@ -645,18 +562,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!healthy) break;
-      if constexpr (kSplit) {
-        healthy = join_halves(sum, half, quarter, warp - 4, lane, rank, share, splits, rounds, shared + kStore, base + kStore, ready,
-                              released, [&](int row, int col, const float4& total) {
-                                int row_tile, col_tile;
-                                tile_at(tile, row_tile, col_tile);
-                                const int t = (row_tile * 2 + rank) * kRows + row, o = col_tile * kCols + col;
-                                if (t < tokens && o < out_features)
-                                  *reinterpret_cast<uint2*>(out + static_cast<size_t>(t) * out_features + o) =
-                                      make_uint2(pack_bf16x2(total.x, total.y), pack_bf16x2(total.z, total.w));
-                              });
-        continue;
-      }
       // The warp's 32 rows x 128 outputs leave through its own 8 KB (swizzled as the copy reads them), so that the next
       // tile's additions start at once: all SMs end a tile together, and plain stores held them up for 3000 cycles.
       int row_tile, col_tile;
@@ -685,11 +590,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncwarp();
   fence_before_sync();
   __syncthreads();
-  cluster_sync();  // neither CTA's memory is in use by the other any more
+  cluster_arrive();
+  cluster_wait();  // no CTA's memory is in use by another any more
   if (warp == 2)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kBuffers * kHalf) : "memory");
   __syncwarp();
-  cluster_sync();
+  cluster_arrive();
+  cluster_wait();
 }
 
 }  // namespace pair
@@ -709,11 +616,11 @@ struct Shape {
   static constexpr int kMine = COLS / (kAdders / 4);              // tokens of one adding warp
   static constexpr int kThreads = 128 + 32 * kAdders;
   static constexpr int kStageBytes = (kRows + COLS) * kRowBytes;
-  static constexpr int kStages = COLS == 16 ? 11 : COLS == 32 ? 10 : COLS == 64 ? 7 : 4;
+  static constexpr int kStages = COLS == 16 ? 11 : COLS == 32 ? 9 : COLS == 64 ? 7 : 4;
   static constexpr int kSlots = COLS == 128 ? 8 : 16;             // of scales, one per block in flight
   static constexpr int kSlotFloats = COLS + 4;                    // the tokens' scales, the weight block's, 3 unused
-  static constexpr int kPartial = kStages * kStageBytes;          // [from][own token][output row] FP32, pushed by the cluster
-  static constexpr int kScales = kPartial + (COLS + kMaxSplits) * kRows * 4;
+  static constexpr int kPartial = kStages * kStageBytes;          // [from][own group][output row] of four tokens' FP32 sums
+  static constexpr int kScales = kPartial + (COLS / 4 + kMaxSplits) * kRows * 16;
   static constexpr int kBarriers = kScales + kSlots * kSlotFloats * 4;
   static constexpr int kShared = 1024 + kBarriers + 256;
   static constexpr int kColumns = 2 * COLS;                       // of tensor memory
@@ -721,8 +628,8 @@ struct Shape {
   static_assert(16 * kStages + 52 <= 256 && kShared <= 232448, "shared memory of one CTA");
 };
 
-// The cluster's CTAs share the blocks of K of one tile.  Token t's sums belong to rank t % splits: everybody pushes them into
-// that CTA's shared memory, the pushes complete on its barrier, and it adds them in rank order.  (Sums left in place and
+// The cluster's CTAs share the blocks of K of one tile.  The sums of tokens 4 g to 4 g + 3 belong to rank g % splits:
+// everybody pushes them into that CTA's shared memory, the pushes complete on its barrier, and it adds them in rank order.  (Sums left in place and
 // read by the others took two fences at cluster scope for each tile, a microsecond each.)
 template <int COLS>
 __global__ void __launch_bounds__(Shape<COLS>::kThreads, 1)
@@ -833,7 +740,7 @@ __global__ void __launch_bounds__(Shape<COLS>::kThreads, 1)
     const int quarter = warp & 3, row = quarter * 32 + lane, col0 = ((warp - 4) >> 2) * kMine;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + col0;
     const float* scales = reinterpret_cast<const float*>(shared + S::kScales);
-    float* partial = reinterpret_cast<float*>(shared + S::kPartial);
+    const float4* partial = reinterpret_cast<const float4*>(shared + S::kPartial);
     int step = 0, done = 0;
     bool entered = false;  // into the cluster: its barriers exist
     for (int tile = cluster; tile < tiles; tile += clusters, ++done) {
@@ -872,16 +779,19 @@ __global__ void __launch_bounds__(Shape<COLS>::kThreads, 1)
       }
       if (!healthy) break;
       const int row0 = tile / token_tiles * kRows, token0 = tile % token_tiles * COLS, visible = min(COLS, tokens - token0);
-      const int per = (COLS + splits - 1) / splits, own = (visible + splits - 1 - rank) / splits;  // tokens of a rank; of this one here
-      if (warp == 4 && lane == 0) barrier_expect(ready, static_cast<uint32_t>(splits * own * kRows * 4));
+      const int groups = (visible + 3) / 4, per = (COLS / 4 + splits - 1) / splits;
+      const int own = (groups + splits - 1 - rank) / splits;  // groups of this rank
+      if (warp == 4 && lane == 0) barrier_expect(ready, static_cast<uint32_t>(splits * own * kRows * 16));
       // (the first pushes wait until every CTA of the cluster has its barriers, the others until the last sums were read)
       if (!entered) cluster_wait();
       entered = true;
       if (done > 0 && !(healthy = wait_warp(released, (done - 1) & 1))) break;
-      int owner = col0 % splits, place = rank * per + col0 / splits;
+      int owner = col0 / 4 % splits, place = rank * per + col0 / 4 / splits;
 #pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        if (col0 + i < visible) push(at_rank(base + S::kPartial + (place * kRows + row) * 4, owner), sum[i], at_rank(ready, owner));
+      for (int i = 0; i < kMine; i += 4) {
+        if (col0 + i < visible)
+          push(at_rank(base + S::kPartial + (place * kRows + row) * 16, owner), make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]),
+               at_rank(ready, owner));
         if (++owner == splits) {
           owner = 0;
           ++place;
@@ -889,14 +799,21 @@ __global__ void __launch_bounds__(Shape<COLS>::kThreads, 1)
       }
       __syncwarp();
       if (!(healthy = wait_warp(ready, done & 1))) break;
-      for (int item = threadIdx.x - 128; item < own * (kRows / 4); item += kAdding) {  // (own token, four outputs)
-        const int t = item / (kRows / 4), r = item % (kRows / 4) * 4;
-        float4 total = *reinterpret_cast<const float4*>(partial + t * kRows + r);
-        for (int from = 1; from < splits; ++from)
-          total = add4(total, *reinterpret_cast<const float4*>(partial + (from * per + t) * kRows + r));
-        if (row0 + r < out_features)
-          *reinterpret_cast<uint2*>(out + static_cast<size_t>(token0 + t * splits + rank) * out_features + row0 + r) =
-              make_uint2(pack_bf16x2(total.x, total.y), pack_bf16x2(total.z, total.w));
+      for (int item = threadIdx.x - 128; item < own * (kRows / 2); item += kAdding) {  // (own group, two outputs)
+        const int group = item / (kRows / 2), r = item % (kRows / 2) * 2;
+        float4 even = make_float4(0.0f, 0.0f, 0.0f, 0.0f), odd = even;
+        for (int from = 0; from < splits; ++from) {
+          const float4* at = partial + (from * per + group) * kRows + r;
+          even = add4(even, at[0]);
+          odd = add4(odd, at[1]);
+        }
+        const int t = (group * splits + rank) * 4;
+        const uint32_t two[4] = {pack_bf16x2(even.x, odd.x), pack_bf16x2(even.y, odd.y), pack_bf16x2(even.z, odd.z),
+                                 pack_bf16x2(even.w, odd.w)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (t + i < visible && row0 + r < out_features)
+            st_u32(out + static_cast<size_t>(token0 + t + i) * out_features + row0 + r, two[i]);
       }
       __syncwarp();
       if (lane < splits) arrive_remote(at_rank(released, lane));
@@ -977,20 +894,18 @@ struct Problem {
   cudaStream_t stream;
 };
 
-template <int COLS>
 int launch_panel(const Problem& p) {
-  using S = panel::Shape<COLS>;
-  constexpr auto kernel = panel::block_gemm_panel_kernel<COLS>;
-  const int status = prepare_kernel<kernel>(S::kShared, panel::kLaunchRegisters);
+  constexpr auto kernel = panel::block_gemm_panel_kernel;
+  const int status = prepare_kernel<kernel>(panel::kShared, panel::kLaunchRegisters);
   if (status != host::kOk) return status;
   CUtensorMap a, w;
   if (!encode_codes(&a, p.activations, p.tokens, p.in_features, panel::kRows) ||
-      !encode_codes(&w, p.weights, p.out_features, p.in_features, COLS))
+      !encode_codes(&w, p.weights, p.out_features, p.in_features, panel::kCols))
     return host::kNotSupported;
-  const int row_tiles = (p.tokens + panel::kRows - 1) / panel::kRows, col_tiles = (p.out_features + COLS - 1) / COLS;
+  const int row_tiles = (p.tokens + panel::kRows - 1) / panel::kRows, col_tiles = (p.out_features + panel::kCols - 1) / panel::kCols;
   if (static_cast<long long>(row_tiles) * col_tiles > 0x7fffffff / 2) return host::kNotSupported;
   const int tiles = row_tiles * col_tiles, sms = host::current_device_sm_count();
-  host::launch_kernel(kernel, dim3(tiles < sms ? tiles : sms), dim3(panel::kThreads), S::kShared, p.stream, true, a, w,
+  host::launch_kernel(kernel, dim3(tiles < sms ? tiles : sms), dim3(panel::kThreads), panel::kShared, p.stream, true, a, w,
                       p.activation_scales, p.weight_scales, p.tokens, p.out_features, p.blocks, row_tiles, col_tiles, p.out);
   return host::launch_status();
 }
@@ -1043,9 +958,8 @@ int launch_clusters(const Problem& p, int size, int clusters, int threads, int s
   return host::launch_status();
 }
 
-template <bool kSplit>
-int launch_pair(const Problem& p, int splits) {
-  constexpr auto kernel = pair::block_gemm_pair_kernel<kSplit>;
+int launch_pair(const Problem& p) {
+  constexpr auto kernel = pair::block_gemm_pair_kernel;
   const int status = prepare_kernel<kernel>(pair::kShared, pair::kLaunchRegisters);
   if (status != host::kOk) return status;
   CUtensorMap a, w, o;
@@ -1055,10 +969,9 @@ int launch_pair(const Problem& p, int splits) {
     return host::kNotSupported;
   const int row_tiles = (p.tokens + 2 * pair::kRows - 1) / (2 * pair::kRows), col_tiles = (p.out_features + pair::kCols - 1) / pair::kCols;
   if (static_cast<long long>(row_tiles) * col_tiles > 0x7fffffff / 2) return host::kNotSupported;
-  const int tiles = row_tiles * col_tiles, resident = resident_clusters<kernel, pair::kThreads>(2 * splits, pair::kShared);
-  return launch_clusters<kernel>(p, 2 * splits, tiles < resident ? tiles : resident, pair::kThreads, pair::kShared, a, w, o,
-                                 p.activation_scales, p.weight_scales, p.tokens, p.out_features, p.blocks, row_tiles, col_tiles,
-                                 splits, p.out);
+  const int tiles = row_tiles * col_tiles, resident = resident_clusters<kernel, pair::kThreads>(2, pair::kShared);
+  return launch_clusters<kernel>(p, 2, tiles < resident ? tiles : resident, pair::kThreads, pair::kShared, a, w, o,
+                                 p.activation_scales, p.weight_scales, p.tokens, p.out_features, p.blocks, row_tiles, col_tiles);
 }
 
 template <int COLS>
@@ -1128,7 +1041,7 @@ extern "C" int q3x_b200_fp8_block_gemm_bf16(const uint8_t* weights, const float*
   if (tokens <= 128) return launch_strip<128>(p);
   // 256 outputs per tile where that still gives every SM a tile
   const size_t wide_tiles = (tokens + 127) / 128 * ((out_features + 255) / 256);
-  return wide_tiles >= static_cast<size_t>(current_device_sm_count()) ? launch_pair<false>(p, 1) : launch_panel<128>(p);
+  return wide_tiles >= static_cast<size_t>(current_device_sm_count()) ? launch_pair(p) : launch_panel(p);
 }
 
 extern "C" int q3x_b200_fp8_block_gemm_error(void) {

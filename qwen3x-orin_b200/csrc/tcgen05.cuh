@@ -102,16 +102,16 @@ __device__ __forceinline__ void mma_e4m3(uint32_t accumulator, uint64_t a, uint6
 }
 
 // The same on a pair of CTAs: M = 256, each CTA holds 128 rows of A and of the accumulator and n / 2 rows of B, at the
-// same offsets; the leader (the even rank of the two) issues, and a commit arrives on both CTAs' copies of the barrier.
+// same offsets; the leader (rank 0 of the cluster) issues, and a commit arrives on both CTAs' copies of the barrier.
 __device__ __forceinline__ void mma_e4m3_pair(uint32_t accumulator, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(accumulator),
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void commit_pair(uint32_t barrier, int leader) {
+__device__ __forceinline__ void commit_pair(uint32_t barrier) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(barrier),
-               "h"(static_cast<uint16_t>(3 << leader))
+               "h"(static_cast<uint16_t>(3))
                : "memory");
 }
 // One lane of a converged warp, always the same one.  A warp that issues walks its loop with all lanes and lets this one
@@ -134,6 +134,7 @@ __device__ __forceinline__ void barrier_expect(uint32_t barrier, uint32_t bytes)
 __device__ __forceinline__ void barrier_arrive(uint32_t barrier) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(barrier) : "memory");
 }
+// Whether the phase is complete; one that is not may hold the warp, until it is or for some microseconds.
 __device__ __forceinline__ bool barrier_try(uint32_t barrier, uint32_t parity) {
   uint32_t done;
   asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"

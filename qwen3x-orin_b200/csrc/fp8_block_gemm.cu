@@ -903,14 +903,13 @@ int launch_panel(const Problem& p) {
       !encode_codes(&w, p.weights, p.out_features, p.in_features, panel::kCols))
     return host::kNotSupported;
   const int row_tiles = (p.tokens + panel::kRows - 1) / panel::kRows, col_tiles = (p.out_features + panel::kCols - 1) / panel::kCols;
-  if (static_cast<long long>(row_tiles) * col_tiles > 0x7fffffff / 2) return host::kNotSupported;
   const int tiles = row_tiles * col_tiles, sms = host::current_device_sm_count();
   host::launch_kernel(kernel, dim3(tiles < sms ? tiles : sms), dim3(panel::kThreads), panel::kShared, p.stream, true, a, w,
                       p.activation_scales, p.weight_scales, p.tokens, p.out_features, p.blocks, row_tiles, col_tiles, p.out);
   return host::launch_status();
 }
 
-// Clusters of `splits` CTAs that are resident at once (one CTA per SM; a cluster lives inside one group of SMs, so that
+// Clusters of `splits` CTAs of a prepared kernel that are resident at once (one CTA per SM; a cluster lives inside one group of SMs, so that
 // sizes that do not divide the groups leave SMs idle: 74 of two, 45 of three, 33 of four, 15 of seven or eight).
 template <auto kKernel, int kThreads>
 int resident_clusters(int splits, int shared) {
@@ -968,10 +967,31 @@ int launch_pair(const Problem& p) {
       !encode_map(&o, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.out, p.tokens, p.out_features, 32))
     return host::kNotSupported;
   const int row_tiles = (p.tokens + 2 * pair::kRows - 1) / (2 * pair::kRows), col_tiles = (p.out_features + pair::kCols - 1) / pair::kCols;
-  if (static_cast<long long>(row_tiles) * col_tiles > 0x7fffffff / 2) return host::kNotSupported;
   const int tiles = row_tiles * col_tiles, resident = resident_clusters<kernel, pair::kThreads>(2, pair::kShared);
   return launch_clusters<kernel>(p, 2, tiles < resident ? tiles : resident, pair::kThreads, pair::kShared, a, w, o,
                                  p.activation_scales, p.weight_scales, p.tokens, p.out_features, p.blocks, row_tiles, col_tiles);
+}
+
+// How a strip's tiles are shared out: the number of CTAs per tile with the fewest blocks on the busiest one, a tile's end
+// (pushing and adding the sums, the more tokens the longer) counted as kEnd blocks.
+struct StripPlan {
+  int tiles, token_tiles, splits, clusters;
+  long long rounds, blocks;  // tiles one after the other on the busiest CTA, and the blocks of one of them
+};
+template <int COLS>
+StripPlan plan_strip(const Problem& p) {
+  using S = strip::Shape<COLS>;
+  constexpr auto kernel = strip::block_gemm_strip_kernel<COLS>;
+  constexpr int kEnd = 2 + COLS / 32;
+  StripPlan best{};
+  const int token_tiles = (p.tokens + COLS - 1) / COLS, tiles = (p.out_features + strip::kRows - 1) / strip::kRows * token_tiles;
+  for (int splits = 1; splits <= strip::kMaxSplits && splits <= p.blocks; ++splits) {
+    const int resident = resident_clusters<kernel, S::kThreads>(splits, S::kShared);
+    const long long rounds = (tiles + resident - 1) / resident, blocks = (p.blocks + splits - 1) / splits;
+    if (best.splits == 0 || rounds * (blocks + kEnd) < best.rounds * (best.blocks + kEnd))
+      best = StripPlan{tiles, token_tiles, splits, tiles < resident ? tiles : resident, rounds, blocks};
+  }
+  return best;
 }
 
 template <int COLS>
@@ -984,25 +1004,28 @@ int launch_strip(const Problem& p) {
   if (!encode_codes(&a, p.activations, p.tokens, p.in_features, COLS) ||
       !encode_codes(&w, p.weights, p.out_features, p.in_features, strip::kRows))
     return host::kNotSupported;
-  const int out_tiles = (p.out_features + strip::kRows - 1) / strip::kRows, token_tiles = (p.tokens + COLS - 1) / COLS;
-  if (static_cast<long long>(out_tiles) * token_tiles > 0x7fffffff / 2) return host::kNotSupported;
-  const int tiles = out_tiles * token_tiles;
-  // CTAs that share a tile's blocks of K: the count with the fewest blocks on the busiest CTA, joining the sums counted
-  // as kJoin blocks
-  constexpr double kJoin = 3.0;
-  int splits = 1, clusters = 1;
-  double least = 1e300;
-  for (int s = 1; s <= strip::kMaxSplits && s <= p.blocks; ++s) {
-    const int resident = resident_clusters<kernel, S::kThreads>(s, S::kShared);
-    const double time = static_cast<double>((tiles + resident - 1) / resident) * ((p.blocks + s - 1) / s) + (s > 1 ? kJoin : 0.0);
-    if (time < least) {
-      least = time;
-      splits = s;
-      clusters = tiles < resident ? tiles : resident;
-    }
+  const StripPlan plan = plan_strip<COLS>(p);
+  return launch_clusters<kernel>(p, plan.splits, plan.clusters, S::kThreads, S::kShared, a, w, p.activation_scales,
+                                 p.weight_scales, p.tokens, p.out_features, p.blocks, plan.token_tiles, plan.tiles, plan.splits, p.out);
+}
+
+// More than 64 tokens: the kernel with the least time by what each was measured to take, in hundredths of a microsecond:
+// a fixed part, then for every round of tiles on the busiest CTA so much per block of K -- panels 3 + 0.28 us
+// (128 x 5120 x 17408: 40.6 us, pairs 54.6, strips 29.2), pairs 4.5 + 0.40 us (2048 x 10240 x 5120: 89 us, panels 118), strips
+// of 128 tokens 3.6 + 0.48 us and 3.5 us for the sums of a tile (128 x 5120 x 5120: 13.9 us, panels 14.4, pairs 20.0).
+int launch_many(const Problem& p) {
+  const long long sms = host::current_device_sm_count(), pairs = sms / 2 > 0 ? sms / 2 : 1;
+  auto tiles = [&](long long rows, long long cols) { return (p.tokens + rows - 1) / rows * ((p.out_features + cols - 1) / cols); };
+  const long long panel_time = 300 + (tiles(panel::kRows, panel::kCols) + sms - 1) / sms * p.blocks * 28;
+  const long long pair_time = 450 + (tiles(2 * pair::kRows, pair::kCols) + pairs - 1) / pairs * p.blocks * 40;
+  if (p.tokens <= 128) {
+    const int status = prepare_kernel<strip::block_gemm_strip_kernel<128>>(strip::Shape<128>::kShared, 0);
+    if (status != host::kOk) return status;
+    const StripPlan plan = plan_strip<128>(p);
+    const long long strip_time = 360 + plan.rounds * (plan.blocks * 48 + 350);
+    if (strip_time < panel_time && strip_time < pair_time) return launch_strip<128>(p);
   }
-  return launch_clusters<kernel>(p, splits, clusters, S::kThreads, S::kShared, a, w, p.activation_scales, p.weight_scales, p.tokens,
-                                 p.out_features, p.blocks, token_tiles, tiles, splits, p.out);
+  return panel_time <= pair_time ? launch_panel(p) : launch_pair(p);
 }
 
 }  // namespace
@@ -1032,16 +1055,15 @@ extern "C" int q3x_b200_fp8_block_gemm_bf16(const uint8_t* weights, const float*
   if (!aligned16(weights) || !aligned16(activations) || !aligned16(out) ||
       (reinterpret_cast<uintptr_t>(weight_scales) & 3u) != 0 || (reinterpret_cast<uintptr_t>(activation_scales) & 3u) != 0)
     return kNotSupported;
+  // (tiles are counted in 32 bits)
+  if (((tokens + 15) / 16) * ((out_features + 127) / 128) > 0x7fffffffu / 2) return kNotSupported;
   clear_stale_error();
   const Problem p{weights, activations, weight_scales, activation_scales, static_cast<int>(tokens), static_cast<int>(out_features),
                   static_cast<int>(in_features), static_cast<int>(blocks), out, as_stream(stream)};
   if (tokens <= 16) return launch_strip<16>(p);
   if (tokens <= 32) return launch_strip<32>(p);
   if (tokens <= 64) return launch_strip<64>(p);
-  if (tokens <= 128) return launch_strip<128>(p);
-  // 256 outputs per tile where that still gives every SM a tile
-  const size_t wide_tiles = (tokens + 127) / 128 * ((out_features + 255) / 256);
-  return wide_tiles >= static_cast<size_t>(current_device_sm_count()) ? launch_pair(p) : launch_panel(p);
+  return launch_many(p);
 }
 
 extern "C" int q3x_b200_fp8_block_gemm_error(void) {

@@ -13,6 +13,8 @@
 // Every kernel is a stream that reads its operands once.  A lane owns eight neighbouring columns (one 128-bit load per
 // operand, one 64-bit store of codes), sixteen lanes own a block, so a block's amax takes four shuffles and nothing leaves
 // registers between the arithmetic and the codes.
+#include <type_traits>
+
 #include "device_utils.cuh"
 #include "host_checks.hpp"
 #include "internal.hpp"
@@ -77,64 +79,76 @@ struct FromSiluMul {  // first operand = gate, second = up
 
 constexpr int kThreads = 256;
 
-// CTA (row, split): vectors split * 256 + thread, stepping by gridDim.y * 256, of one row.
-template <class Source>
+// kPerRow threads of a CTA share a row (a power of two, so that narrow rows do not leave a CTA idle: 8192 x 256 took 9 us
+// with a CTA per row), each with kDepth vectors of every operand in flight; the grid's second dimension splits wide rows
+// when there are few of them.
+template <class Source, int kPerRow, int kDepth>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const uint16_t* __restrict__ a, const uint16_t* __restrict__ b,
                                                                  size_t row_stride, size_t rows, int row_vectors,
                                                                  uint8_t* __restrict__ codes, float* __restrict__ scales) {
   release_next_kernel();
   wait_for_prior_kernels();
-  const size_t row = blockIdx.x;
+  const size_t row = static_cast<size_t>(blockIdx.x) * (kThreads / kPerRow) + threadIdx.x / kPerRow;
+  const int lane = threadIdx.x % kPerRow, step = gridDim.y * kPerRow;
+  const bool live = row < rows;
   const uint16_t* a_row = a + row * row_stride;
   const uint16_t* b_row = Source::kTwoInputs ? b + row * row_stride : nullptr;
   uint8_t* code_row = codes + row * static_cast<size_t>(row_vectors) * 8;
-  const int lane = threadIdx.x & 31;
-  // (the bound is that of the warp's first lane, so that all lanes take part in the shuffles)
-  for (int first = blockIdx.y * kThreads + (threadIdx.x & ~31); first < row_vectors; first += gridDim.y * kThreads) {
-    const int v = first + lane;
-    const bool valid = v < row_vectors;
-    uint4 x = make_uint4(0, 0, 0, 0), z = make_uint4(0, 0, 0, 0);
-    if (valid) {
-      x = ld_stream(a_row + static_cast<size_t>(v) * 8);
-      if (Source::kTwoInputs) z = ld_stream(b_row + static_cast<size_t>(v) * 8);
+  // (a whole warp makes the same turns, whatever its lanes' last vector: all of them take part in the shuffles)
+  for (int first = blockIdx.y * kPerRow; first < row_vectors; first += kDepth * step) {
+    uint4 x[kDepth], z[kDepth];
+#pragma unroll
+    for (int k = 0; k < kDepth; ++k) {
+      const int v = first + k * step + lane;
+      x[k] = z[k] = make_uint4(0, 0, 0, 0);
+      if (live && v < row_vectors) {
+        x[k] = ld_stream(a_row + static_cast<size_t>(v) * 8);
+        if (Source::kTwoInputs) z[k] = ld_stream(b_row + static_cast<size_t>(v) * 8);
+      }
     }
-    float y[8];
-    Source::apply(x, z, y);
-    const float scale = scale_of_amax(block_amax(finite_amax8(y)));
-    if (valid) {
-      *reinterpret_cast<uint2*>(code_row + static_cast<size_t>(v) * 8) = encode8(y, __frcp_rn(scale));
-      if ((lane & (kBlockLanes - 1)) == 0) scales[static_cast<size_t>(v / kBlockLanes) * rows + row] = scale;
+#pragma unroll
+    for (int k = 0; k < kDepth; ++k) {
+      const int v = first + k * step + lane;
+      if (first + k * step >= row_vectors) break;
+      float y[8];
+      Source::apply(x[k], z[k], y);
+      const float scale = scale_of_amax(block_amax(finite_amax8(y)));
+      if (live && v < row_vectors) {
+        *reinterpret_cast<uint2*>(code_row + static_cast<size_t>(v) * 8) = encode8(y, __frcp_rn(scale));
+        if ((lane & (kBlockLanes - 1)) == 0) scales[static_cast<size_t>(v / kBlockLanes) * rows + row] = scale;
+      }
     }
   }
 }
 
-// One CTA per row; the row stays in registers between the sum of squares and the codes.
-template <int THREADS, int VPT>
-__global__ void __launch_bounds__(THREADS) residual_norm_fp8_kernel(const uint16_t* left, const uint16_t* right,
-                                                                    const uint16_t* __restrict__ weight, size_t rows,
-                                                                    int row_vectors, float inv_width, float eps,
-                                                                    uint16_t* residual_out, uint16_t* normalized_out,
-                                                                    bool coherent, uint8_t* __restrict__ codes,
-                                                                    float* __restrict__ scales) {
-  __shared__ float scratch[THREADS / 32];
+// One CTA per row, kDepth vectors per thread; the row stays in registers between the sum of squares and the codes, and the
+// weights are requested with it.
+constexpr int kMostThreads = 512;
+template <int kDepth>
+__global__ void __launch_bounds__(kDepth == 1 ? 1024 : kMostThreads)
+    residual_norm_fp8_kernel(const uint16_t* left, const uint16_t* right, const uint16_t* __restrict__ weight, size_t rows,
+                             int row_vectors, float inv_width, float eps, uint16_t* residual_out, uint16_t* normalized_out,
+                             bool coherent, uint8_t* __restrict__ codes, float* __restrict__ scales) {
+  __shared__ float scratch[32];
   release_next_kernel();
   wait_for_prior_kernels();
   const size_t row = blockIdx.x;
   const size_t base = row * static_cast<size_t>(row_vectors) * 8;
-  uint4 x[VPT], r[VPT];
+  uint4 x[kDepth], r[kDepth], w[kDepth];
 #pragma unroll
-  for (int k = 0; k < VPT; ++k) {
-    const int v = threadIdx.x + k * THREADS;
-    x[k] = r[k] = make_uint4(0, 0, 0, 0);
+  for (int k = 0; k < kDepth; ++k) {
+    const int v = threadIdx.x + k * blockDim.x;
+    x[k] = r[k] = w[k] = make_uint4(0, 0, 0, 0);
     if (v < row_vectors) {
       x[k] = ld_stream(left + base + v * 8);
       r[k] = coherent ? ld_vec(right + base + v * 8) : ld_stream(right + base + v * 8);
+      w[k] = ld_weight(weight + v * 8);
     }
   }
   float partial = 0.0f;
 #pragma unroll
-  for (int k = 0; k < VPT; ++k) {
-    const int v = threadIdx.x + k * THREADS;
+  for (int k = 0; k < kDepth; ++k) {
+    const int v = threadIdx.x + k * blockDim.x;
     float l[8], rr[8];
     unpack8(x[k], l);
     unpack8(r[k], rr);
@@ -143,16 +157,19 @@ __global__ void __launch_bounds__(THREADS) residual_norm_fp8_kernel(const uint16
     if (v < row_vectors) st_vec(residual_out + base + v * 8, x[k]);
     partial += sum_squares8(x[k]);
   }
-  const float inv = inverse_rms(block_sum<THREADS / 32>(partial, scratch), inv_width, eps);
+  // the sum over the CTA's warps, in the same order in every thread
+  partial = group_sum<32>(partial);
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = partial;
+  __syncthreads();
+  float total = 0.0f;
+  for (int i = 0; i < blockDim.x / 32; ++i) total += scratch[i];
+  const float inv = inverse_rms(total, inv_width, eps);
 #pragma unroll
-  for (int k = 0; k < VPT; ++k) {
-    const int v = threadIdx.x + k * THREADS;
-    const bool valid = v < row_vectors;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (valid) w = ld_weight(weight + v * 8);
+  for (int k = 0; k < kDepth; ++k) {
+    const int v = threadIdx.x + k * blockDim.x;
     float y[8], wf[8];
     unpack8(x[k], y);
-    unpack8(w, wf);
+    unpack8(w[k], wf);
     const float2 inv2 = make_float2(inv, inv);
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
@@ -163,7 +180,7 @@ __global__ void __launch_bounds__(THREADS) residual_norm_fp8_kernel(const uint16
     }
     // (a lane past the row's end holds 0 * inv: not NaN unless the row's own sum is, and then fmaxf drops it)
     const float scale = scale_of_amax(block_amax(finite_amax8(y)));
-    if (valid) {
+    if (v < row_vectors) {
       if (normalized_out != nullptr) st_vec(normalized_out + base + v * 8, pack8(y));
       *reinterpret_cast<uint2*>(codes + base + v * 8) = encode8(y, __frcp_rn(scale));
       if ((threadIdx.x & (kBlockLanes - 1)) == 0) scales[static_cast<size_t>(v / kBlockLanes) * rows + row] = scale;
@@ -186,38 +203,55 @@ bool codes_aligned(const uint8_t* codes, const float* scales) {
   return host::aligned16(codes) && (reinterpret_cast<uintptr_t>(scales) & 3u) == 0;
 }
 
+template <class Source, int kPerRow, int kDepth>
+void launch_quantize_deep(const uint16_t* a, const uint16_t* b, size_t row_stride, size_t rows, int row_vectors, uint8_t* codes,
+                             float* scales, cudaStream_t s) {
+  constexpr auto kernel = quantize_rows_kernel<Source, kPerRow, kDepth>;
+  const size_t ctas = (rows + kThreads / kPerRow - 1) / (kThreads / kPerRow), chunks = (row_vectors + kPerRow - 1) / kPerRow;
+  const size_t resident = host::resident_grid(kernel, kThreads);
+  size_t splits = ctas >= resident ? 1 : (resident + ctas - 1) / ctas;
+  if (splits > chunks) splits = chunks;
+  host::launch_kernel(kernel, dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(splits)), dim3(kThreads), 0, s,
+                      host::latency_bound_launch(ctas * splits), a, b, row_stride, rows, row_vectors, codes, scales);
+}
+
+// Three vectors in flight per thread once the rows alone fill the GPU (8192 x 6144: 26.9 us; one 30.3, two 29.0, four 29.1;
+// SwiGLU of 8192 x 17408: 122.5 us; 125.9, 128.9, 134.4), one while they do not (333 x 6144: 2.9 us, as with three; SwiGLU of
+// 1 x 17408 1.43 us against 1.52).
+template <class Source, int kPerRow>
+void launch_quantize_per_row(const uint16_t* a, const uint16_t* b, size_t row_stride, size_t rows, int row_vectors, uint8_t* codes,
+                             float* scales, cudaStream_t s) {
+  if (rows / (kThreads / kPerRow) >= host::resident_grid(quantize_rows_kernel<Source, kPerRow, 3>, kThreads))
+    launch_quantize_deep<Source, kPerRow, 3>(a, b, row_stride, rows, row_vectors, codes, scales, s);
+  else
+    launch_quantize_deep<Source, kPerRow, 1>(a, b, row_stride, rows, row_vectors, codes, scales, s);
+}
+
 template <class Source>
 int launch_quantize_rows(const uint16_t* a, const uint16_t* b, size_t row_stride, size_t rows, size_t cols, uint8_t* codes,
                          float* scales, void* stream) {
   using namespace host;
-  const int row_vectors = static_cast<int>(cols / 8);
-  const size_t chunks = (static_cast<size_t>(row_vectors) + kThreads - 1) / kThreads;
-  const size_t resident = resident_grid(quantize_rows_kernel<Source>, kThreads);
-  size_t splits = rows >= resident ? 1 : (resident + rows - 1) / rows;
-  if (splits > chunks) splits = chunks;
+  const int vectors = static_cast<int>(cols / 8);
+  cudaStream_t s = as_stream(stream);
   clear_stale_error();
-  launch_kernel(quantize_rows_kernel<Source>, dim3(static_cast<unsigned>(rows), static_cast<unsigned>(splits)), dim3(kThreads), 0,
-                as_stream(stream), latency_bound_launch(rows * splits), a, b, row_stride, rows, row_vectors, codes, scales);
+  if (vectors <= 16) launch_quantize_per_row<Source, 16>(a, b, row_stride, rows, vectors, codes, scales, s);
+  else if (vectors <= 64) launch_quantize_per_row<Source, 64>(a, b, row_stride, rows, vectors, codes, scales, s);
+  else if (vectors <= 128) launch_quantize_per_row<Source, 128>(a, b, row_stride, rows, vectors, codes, scales, s);
+  else launch_quantize_per_row<Source, 256>(a, b, row_stride, rows, vectors, codes, scales, s);
   return launch_status();
 }
 
-template <int THREADS>
-void launch_residual_norm(int vpt, size_t rows, cudaStream_t s, const uint16_t* left, const uint16_t* right,
-                          const uint16_t* weight, int row_vectors, float inv_width, float eps, uint16_t* residual_out,
-                          uint16_t* normalized_out, bool coherent, uint8_t* codes, float* scales) {
-#define Q3X_CASE(V)                                                                                                         \
-  case V:                                                                                                                   \
-    host::launch_kernel(residual_norm_fp8_kernel<THREADS, V>, dim3(static_cast<unsigned>(rows)), dim3(THREADS), 0, s,     \
-                        host::latency_bound_launch(rows), left, right, weight, rows, row_vectors, inv_width, eps,         \
-                        residual_out, normalized_out, coherent, codes, scales);                                           \
-    break;
-  switch (vpt) {
-    Q3X_CASE(1) Q3X_CASE(2) Q3X_CASE(3) Q3X_CASE(4) Q3X_CASE(5) Q3X_CASE(6) Q3X_CASE(7) Q3X_CASE(8)
-  }
-#undef Q3X_CASE
+template <int kDepth>
+void launch_residual_norm(size_t rows, cudaStream_t s, const uint16_t* left, const uint16_t* right, const uint16_t* weight,
+                          int row_vectors, float inv_width, float eps, uint16_t* residual_out, uint16_t* normalized_out,
+                          bool coherent, uint8_t* codes, float* scales) {
+  const int threads = ((row_vectors + kDepth - 1) / kDepth + 31) / 32 * 32;
+  host::launch_kernel(residual_norm_fp8_kernel<kDepth>, dim3(static_cast<unsigned>(rows)), dim3(threads), 0, s,
+                      host::latency_bound_launch(rows), left, right, weight, rows, row_vectors, inv_width, eps, residual_out,
+                      normalized_out, coherent, codes, scales);
 }
 
-constexpr size_t kWidestRow = 512 * 8 * 8;  // 512 threads of eight vectors of eight columns
+constexpr size_t kWidestRow = kMostThreads * 8 * 8;  // eight vectors of eight columns per thread
 
 }  // namespace
 }  // namespace q3x
@@ -277,19 +311,17 @@ extern "C" int q3x_b200_residual_add_rms_norm_fp8_block(const uint16_t* left, co
     return kNotSupported;
   clear_stale_error();
   const int row_vectors = static_cast<int>(hidden / 8);
-  const int threads = row_vectors <= 1024 ? 128 : row_vectors <= 2048 ? 256 : 512;
-  const int vpt = (row_vectors + threads - 1) / threads;
   const float inv_width = 1.0f / static_cast<float>(hidden);
   cudaStream_t s = as_stream(stream);
   const bool coherent = normalized_out == right;
-  if (threads == 128)
-    launch_residual_norm<128>(vpt, tokens, s, left, right, weight, row_vectors, inv_width, eps, residual_out, normalized_out,
-                              coherent, codes, scales);
-  else if (threads == 256)
-    launch_residual_norm<256>(vpt, tokens, s, left, right, weight, row_vectors, inv_width, eps, residual_out, normalized_out,
-                              coherent, codes, scales);
-  else
-    launch_residual_norm<512>(vpt, tokens, s, left, right, weight, row_vectors, inv_width, eps, residual_out, normalized_out,
-                              coherent, codes, scales);
+  auto launch = [&](auto depth) {
+    launch_residual_norm<decltype(depth)::value>(tokens, s, left, right, weight, row_vectors, inv_width, eps, residual_out,
+                                                 normalized_out, coherent, codes, scales);
+  };
+  // One vector per thread while the call is bound by latency (1 x 5120: 1.9 us, with three 2.4), three when it streams (8192 x
+  // 5120: 49.0 us; one 57.6, two 50.3, four 51.3), eight for rows beyond that.
+  if (row_vectors <= 64 || (row_vectors <= 1024 && latency_bound_launch(tokens))) launch(std::integral_constant<int, 1>{});
+  else if (row_vectors <= 3 * kMostThreads) launch(std::integral_constant<int, 3>{});
+  else launch(std::integral_constant<int, 8>{});
   return launch_status();
 }

@@ -388,6 +388,62 @@ class ProjectedMlp:
             raise RuntimeError("a bounded wait of a single-kernel NVFP4 operator gave up: outputs are invalid")
 
 
+class ProjectedMlpFp8Block:
+    """One layer's MLP block WITH its projections, both operands of every projection in FP8 with one scale per block of
+    128 (the form in which FP8 checkpoints with block scales hold their weights), for a panel of tokens or a single one:
+
+        residual + RMSNorm + FP8  ->  gate | up = x W^T (one product of the merged weight)  ->  SwiGLU + FP8 of the two
+        halves of its rows  ->  down = h W_down^T
+
+    four kernels.  The weights are synthetic: random matrices, quantised per 128 x 128 block."""
+
+    def __init__(self, tokens: int, device, hidden: int = HIDDEN, intermediate: int = INTERMEDIATE, seed: int = 11):
+        self.tokens, self.hidden, self.intermediate, self.device = tokens, hidden, intermediate, device
+        gen = torch.Generator(device=device).manual_seed(seed)
+        bf = dict(device=device, dtype=torch.bfloat16)
+        u8 = dict(device=device, dtype=torch.uint8)
+        blocks = lambda width: (width + 127) // 128
+
+        def weight(rows, cols):
+            dense = torch.zeros((blocks(rows) * 128, blocks(cols) * 128), device=device)
+            dense[:rows, :cols] = torch.randn((rows, cols), generator=gen, device=device) * 0.03
+            tiles = dense.view(blocks(rows), 128, blocks(cols), 128)
+            scales = tiles.abs().amax(dim=(1, 3)) / 448.0
+            codes = (tiles / scales[:, None, :, None]).clamp(-448.0, 448.0).to(torch.float8_e4m3fn).view(dense.shape)
+            return {"codes": codes[:rows, :cols].contiguous().view(torch.uint8), "scales": scales.contiguous()}
+
+        self.w_gate_up, self.w_down = weight(2 * intermediate, hidden), weight(hidden, intermediate)
+        rand = lambda shape, std=1.0: (torch.randn(shape, generator=gen, device=device) * std).to(torch.bfloat16)
+        self.norm_w = rand((hidden,), 0.02)
+        self.left, self.right = rand((tokens, hidden)), rand((tokens, hidden))
+        self.residual = torch.empty((tokens, hidden), **bf)
+        self.x_codes = torch.empty((tokens, hidden), **u8)
+        self.x_scales = torch.empty((blocks(hidden), tokens), device=device, dtype=torch.float32)
+        self.gate_up = torch.empty((tokens, 2 * intermediate), **bf)
+        self.h_codes = torch.empty((tokens, intermediate), **u8)
+        self.h_scales = torch.empty((blocks(intermediate), tokens), device=device, dtype=torch.float32)
+        self.down = torch.empty((tokens, hidden), **bf)
+
+    def flops(self) -> float:
+        return 2.0 * self.tokens * self.hidden * self.intermediate * 3
+
+    def enqueue(self, stream) -> None:
+        T, H, I = self.tokens, self.hidden, self.intermediate
+        capi.check("q3x_b200_residual_add_rms_norm_fp8_block", self.left, self.right, self.norm_w, T, H, EPS, self.residual, None,
+                   self.x_codes, self.x_scales, stream)
+        capi.check("q3x_b200_fp8_block_gemm_bf16", self.w_gate_up["codes"], self.w_gate_up["scales"], self.x_codes, self.x_scales,
+                   T, 2 * I, H, self.gate_up, stream)
+        capi.check("q3x_b200_silu_mul_fp8_block", self.gate_up, self.gate_up.data_ptr() + 2 * I, 2 * I, T, I, self.h_codes,
+                   self.h_scales, stream)
+        capi.check("q3x_b200_fp8_block_gemm_bf16", self.w_down["codes"], self.w_down["scales"], self.h_codes, self.h_scales, T, H, I,
+                   self.down, stream)
+
+    def check_error(self) -> None:
+        word = capi.lib().q3x_b200_fp8_block_gemm_error()
+        if word != 0:
+            raise RuntimeError(f"a bounded wait of an FP8 block product gave up (error word {word}): outputs are invalid")
+
+
 WIDEN_FP8_FROM_TOKENS = 128
 
 

@@ -1,6 +1,11 @@
 """GPU tests of the FP8 operators with a scale per block of 128, through the C ABI, against their definition in 64 bits
 (tests/fp8_block_util.py): sizes around whole blocks and tiles, blocks of zeros, subnormals, NaN and infinities, strides,
 streams, captured graphs, and the operators in a row as a layer uses them."""
+import importlib
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -180,7 +185,7 @@ def test_silu_mul_non_finite(g):
 SHAPES = [(1, 8, 16), (1, 128, 128), (1, 5120, 5120), (2, 256, 1024), (3, 136, 2064), (16, 264, 144), (17, 128, 272), (31, 5120, 640),
           (33, 1000, 400), (48, 640, 17408), (64, 1024, 5120), (65, 384, 1296), (100, 24, 2048), (127, 520, 640), (128, 5120, 5120),
           (129, 256, 384), (255, 776, 1040), (256, 2048, 512), (300, 640, 6144), (512, 1288, 5120), (513, 136, 2064), (1000, 4104, 528),
-          (2049, 1032, 656)]
+          (2049, 1032, 656), (9000, 1032, 272), (2049, 2040, 2064), (5000, 2600, 400), (4097, 4104, 656)]
 
 
 def run_gemm(g, a, sa, w, sw, stream=None):
@@ -203,7 +208,8 @@ def test_gemm(g, tokens, n, k):
     assert np.max(over) <= 0, f"{np.max(over)} past the tolerance at {np.unravel_index(np.argmax(over), over.shape)}"
 
 
-@pytest.mark.parametrize("tokens,n,k", [(1, 136, 272), (16, 256, 1040), (40, 264, 640), (130, 392, 528), (600, 520, 400)])
+@pytest.mark.parametrize("tokens,n,k", [(1, 136, 272), (16, 256, 1040), (40, 264, 640), (100, 136, 2064), (130, 392, 528), (600, 520, 400),
+                                        (2049, 2040, 2064)])
 def test_gemm_keeps_non_finite_values_to_their_rows_and_columns(g, tokens, n, k):
     """A NaN code, an infinite scale and scales of zero touch the outputs they belong to and no others."""
     rng = np.random.default_rng([tokens, n, k, 29])
@@ -232,11 +238,12 @@ def test_gemm_keeps_non_finite_values_to_their_rows_and_columns(g, tokens, n, k)
     assert np.array_equal(got[~bad], clean[~bad])
 
 
-@pytest.mark.parametrize("tokens", [1, 5, 16, 40, 129, 700])
-def test_gemm_repeats_bit_for_bit(g, tokens):
+@pytest.mark.parametrize("tokens,n,k", [(1, 520, 5136), (5, 520, 5136), (16, 520, 5136), (40, 520, 5136), (100, 520, 5136), (129, 520, 5136),
+                                        (700, 520, 5136), (2049, 2040, 2064)])
+def test_gemm_repeats_bit_for_bit(g, tokens, n, k):
     """Sums are joined in one order, whatever the launch: equal inputs give equal bytes."""
     rng = np.random.default_rng([tokens, 31])
-    a, sa, w, sw = f8.operands(rng, tokens, 520, 5136)
+    a, sa, w, sw = f8.operands(rng, tokens, n, k)
     first = run_gemm(g, a, sa, w, sw)
     for _ in range(3):
         assert np.array_equal(run_gemm(g, a, sa, w, sw), first)
@@ -275,6 +282,95 @@ def test_gemm_on_streams_and_in_graphs(g, tokens):
     graph.replay()
     g.sync()
     assert np.array_equal(outs[0].get(), want[1]) and np.array_equal(outs[1].get(), want[1])
+
+
+def test_gemm_reads_scales_from_any_float_address(g):
+    rng = np.random.default_rng(43)
+    for tokens in (3, 50, 150):
+        a, sa, w, sw = f8.operands(rng, tokens, 264, 656)
+        out = g.empty_like_dev((tokens, 264))
+        g.capi.check("q3x_b200_fp8_block_gemm_bf16", g.Dev(w), g.Dev(sw, misalign=1), g.Dev(a), g.Dev(sa, misalign=3), tokens, 264, 656,
+                     out, None)
+        g.sync()
+        assert np.array_equal(out.get(), run_gemm(g, a, sa, w, sw))
+
+
+FIRST_CALL = """
+import importlib, sys
+import torch
+capi = importlib.import_module("qwen3x-orin_b200").capi
+capi.load()
+for tokens, n, k in ((1, 520, 1040), (100, 136, 2064), (200, 264, 400), (2049, 2040, 2064)):
+    blocks = (k + 127) // 128
+    w, a = torch.full((n, k), 0x38, dtype=torch.uint8, device="cuda"), torch.full((tokens, k), 0x38, dtype=torch.uint8, device="cuda")
+    sw, sa = torch.ones((n + 127) // 128, blocks, device="cuda"), torch.ones(blocks, tokens, device="cuda")
+    out = torch.zeros(tokens, n, dtype=torch.bfloat16, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        capi.check("q3x_b200_fp8_block_gemm_bf16", w, sw, a, sa, tokens, n, k, out, torch.cuda.current_stream().cuda_stream)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert bool((out == torch.tensor(float(k)).bfloat16().item()).all()), (tokens, n, k)
+assert capi.lib().q3x_b200_fp8_block_gemm_error() == 0
+"""
+
+
+def test_gemm_can_be_captured_by_the_first_call_of_a_process(g):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=240)
+    assert done.returncode == 0, done.stdout[-2000:] + done.stderr[-2000:]
+
+
+# ---------------------------------------------------------------------------------------------------- long tensors
+
+
+def random_codes_on_device(rows, cols, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    codes = torch.randint(0, 256, (rows, cols), generator=gen, device="cuda", dtype=torch.uint8)
+    return torch.where((codes & 0x7F) == 0x7F, torch.full_like(codes, 0x3C), codes)
+
+
+@pytest.mark.parametrize("tokens,n,k", [(70001, 34816, 144), (140001, 136, 17408)])
+def test_gemm_beyond_32_bit_offsets(g, tokens, n, k):
+    """More than 2^31 outputs, and more than 2^31 codes: a few rows from every part against their definition."""
+    a, w = random_codes_on_device(tokens, k, 1), random_codes_on_device(n, k, 2)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    sa = torch.rand((f8.blocks_of(k), tokens), generator=gen, device="cuda") * 0.01 + 0.001
+    sw = torch.rand((f8.blocks_of(n), f8.blocks_of(k)), generator=gen, device="cuda") * 0.001 + 0.0001
+    out = torch.zeros((tokens, n), dtype=torch.bfloat16, device="cuda")
+    g.capi.check("q3x_b200_fp8_block_gemm_bf16", w, sw, a, sa, tokens, n, k, out, None)
+    g.sync()
+    rows = torch.tensor([0, 127, 128, tokens // 2, 61681, 61682, tokens - 129, tokens - 2, tokens - 1], device="cuda")
+    host = lambda t: t.cpu().numpy()
+    want, magnitude = f8.product(host(a[rows]), host(sa[:, rows]), host(w), host(sw))
+    got = host(out[rows].double())
+    assert np.all(np.abs(got - want) <= f8.product_tolerance(want, magnitude, k))
+    assert bool((out != 0).any(dim=1).all())  # no row was left out
+
+
+def test_quantisers_beyond_32_bit_offsets(g):
+    rows, cols = 131073, 17408
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.empty((rows, cols), dtype=torch.bfloat16, device="cuda")
+    for first in range(0, rows, 16384):
+        part = x[first:first + 16384]
+        part.copy_(torch.randn(part.shape, generator=gen, device="cuda"))
+    codes = torch.zeros((rows, cols), dtype=torch.uint8, device="cuda")
+    scales = torch.zeros((f8.blocks_of(cols), rows), device="cuda")
+    picked = torch.tensor([0, 1, 61680, 61681, 123361, 123362, rows - 2, rows - 1], device="cuda")
+    values = x[picked].float().cpu().numpy()
+    g.capi.check("q3x_b200_fp8_block_quantize", x, rows, cols, codes, scales, None)
+    g.sync()
+    want, want_scales = f8.quantize(values)
+    assert np.array_equal(scales[:, picked].cpu().numpy(), want_scales)
+    assert np.array_equal(f8.decode(codes[picked].cpu().numpy()), want)
+    # SwiGLU of the two halves of each row: the second half starts at an odd number of blocks
+    half = cols // 2
+    codes, scales = codes[:, :half].contiguous(), torch.zeros((f8.blocks_of(half), rows), device="cuda")
+    g.capi.check("q3x_b200_silu_mul_fp8_block", x, x.data_ptr() + 2 * half, cols, rows, half, codes, scales, None)
+    g.sync()
+    gate, up = values[:, :half].astype(np.float64), values[:, half:].astype(np.float64)
+    assert_codes(codes[picked].cpu().numpy(), scales[:, picked].cpu().numpy(), gate / (1.0 + np.exp(-gate)) * up, 1.1e-5)
 
 
 # ---------------------------------------------------------------------------------------------------- in a row
@@ -326,3 +422,27 @@ def test_mlp_block_in_a_row(g, tokens):
     g.sync()
     for b, e in zip((residual, x_codes, x_scales, merged, h_codes, h_scales, down), eager):
         assert np.array_equal(b.get(), e) and b.guards_intact()
+
+
+@pytest.mark.parametrize("tokens", [1, 300])
+def test_projected_mlp_fp8_block(g, tokens):
+    """chain.ProjectedMlpFp8Block, stage by stage on its own buffers."""
+    chain = importlib.import_module("qwen3x-orin_b200.chain")
+    block = chain.ProjectedMlpFp8Block(tokens, torch.device("cuda", 0), hidden=1280, intermediate=1040, seed=5)
+    block.enqueue(None)
+    g.sync()
+    block.check_error()
+    bits = lambda t: t.view(torch.int16).cpu().numpy().view(np.uint16)
+    host = lambda t: t.cpu().numpy()
+    r = bf16_values(orc.bf16_encode(bf16_values(bits(block.left)) + bf16_values(bits(block.right))))
+    assert np.array_equal(bf16_values(bits(block.residual)), r)
+    r = r.astype(np.float64)
+    y = r / np.sqrt((r * r).mean(axis=1, keepdims=True) + np.float64(np.float32(chain.EPS))) * (1.0 + bf16_values(bits(block.norm_w)).astype(np.float64))
+    assert_codes(host(block.x_codes), host(block.x_scales), y, 2.0 ** -18, "norm")
+    want, mag = f8.product(host(block.x_codes), host(block.x_scales), host(block.w_gate_up["codes"]), host(block.w_gate_up["scales"]))
+    assert np.all(np.abs(bf16_values(bits(block.gate_up)) - want) <= f8.product_tolerance(want, mag, 1280))
+    m = bf16_values(bits(block.gate_up)).astype(np.float64)
+    h = m[:, :1040] / (1.0 + np.exp(-m[:, :1040])) * m[:, 1040:]
+    assert_codes(host(block.h_codes), host(block.h_scales), h, 1.1e-5, "SwiGLU")
+    want, mag = f8.product(host(block.h_codes), host(block.h_scales), host(block.w_down["codes"]), host(block.w_down["scales"]))
+    assert np.all(np.abs(bf16_values(bits(block.down)) - want) <= f8.product_tolerance(want, mag, 1040))

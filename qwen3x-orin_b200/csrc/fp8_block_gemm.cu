@@ -344,12 +344,14 @@ constexpr int kBand = 8;                    // token tiles walked together
 constexpr int kBuffers = 4;                 // accumulators: parity of the block x half
 constexpr int kStageBytes = (kRows + kCols / 2) * kRowBytes;
 constexpr int kStages = 5;
-constexpr int kSlots = 4;                   // of scales
-constexpr int kSlotFloats = kRows + 4;      // the tokens', the two halves' weight blocks', 2 unused
+constexpr int kSlots = 5;                   // of scales
+constexpr int kSlotBytes = (kRows + 2) * 4;  // the tokens', the two halves' weight blocks'
+constexpr int kAhead = 3;                   // blocks that scales are fetched before their products
+static_assert(kSlots >= kAhead + 2, "see the warp that fetches scales");
 constexpr int kStore = kStages * kStageBytes;                  // [adder][2][32 rows][64 outputs] bf16
 constexpr int kScales = kStore + kAdders * 2 * 32 * 128;
-constexpr int kBarriers = kScales + kSlots * kSlotFloats * 4;
-constexpr int kTmemSlot = kBarriers + 8 * (2 * kStages + 2 * kBuffers + 2 * kSlots);
+constexpr int kBarriers = (kScales + kSlots * kSlotBytes + 31) / 32 * 32;  // (the accumulators' come first: see next_block)
+constexpr int kTmemSlot = kBarriers + 8 * (2 * kStages + 2 * kBuffers + kSlots);
 constexpr int kShared = kTmemSlot + 16;
 static_assert(kShared <= 232448, "shared memory of one CTA");
 
@@ -360,8 +362,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                            int col_tiles) {
   extern __shared__ __align__(1024) uint8_t shared[];
   const uint32_t base = shared_address(shared);
-  const uint32_t full = base + kBarriers, empty = full + 8 * kStages, filled = empty + 8 * kStages,
-                 drained = filled + 8 * kBuffers, scaled = drained + 8 * kBuffers, taken = scaled + 8 * kSlots;
+  const uint32_t filled = base + kBarriers, drained = filled + 8 * kBuffers, full = drained + 8 * kBuffers,
+                 empty = full + 8 * kStages, scaled = empty + 8 * kStages;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(shared + kTmemSlot);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, tiles = row_tiles * col_tiles;
@@ -371,17 +373,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_map(&map_w);
     prefetch_map(&map_out);
     for (int s = 0; s < kStages; ++s) {
-      barrier_init(full + 8 * s, 1);    // (the leader's: both CTAs' copies complete on it)
+      // (the leader's: both CTAs' codes complete on it; its own scales' lanes arrive, and the peer's warp 1 for its scales)
+      barrier_init(full + 8 * s, 1 + 32 + 1);
       barrier_init(empty + 8 * s, 2);   // both halves' products
     }
     for (int i = 0; i < kBuffers; ++i) {
       barrier_init(filled + 8 * i, 1);
       barrier_init(drained + 8 * i, kAdders);  // (the leader's: four warps of each CTA)
     }
-    for (int i = 0; i < kSlots; ++i) {
-      barrier_init(scaled + 8 * i, 32);
-      barrier_init(taken + 8 * i, kAdders);
-    }
+    for (int i = 0; i < kSlots; ++i) barrier_init(scaled + 8 * i, 32);
     barrier_init_fence();
   }
   if (warp == 2) {
@@ -437,7 +437,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!wait_warp(full + 8 * (last % kStages), (last / kStages) & 1)) healthy = false;
     } else if (warp == 2) {
       // The scales of a block, copied without passing through registers (a load held in one for two blocks was measured to
-      // hold up the whole warp wherever the compiler moved it).
+      // hold up the whole warp wherever the compiler moved it).  Products wait for them, so that the adding warps need not.
+      // A slot is free again: when step t - kAhead has left its stage, its accumulators had come round, so step
+      // t - kAhead - 2 was drained and its scales read; slot t % kSlots holds a step at least that old.
       const int weight_rows = (out_features + kBlockK - 1) / kBlockK;
       int step = 0;
       for (int tile = pair; tile < tiles && healthy; tile += pairs) {
@@ -447,27 +449,35 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int row0 = (row_tile * 2 + rank) * kRows;
         const float* weight = sw + static_cast<size_t>(min(col_tile * 2 + (lane & 1), weight_rows - 1)) * blocks;
         for (int b = 0; b < blocks; ++b, ++step) {
-          const int slot = step % kSlots;
-          if (step >= kSlots && !(healthy = wait_warp(taken + 8 * slot, (step / kSlots - 1) & 1))) break;
-          const uint32_t at = base + kScales + slot * (kSlotFloats * 4);
+          const int before = step - kAhead;
+          if (before >= 0 && !(healthy = wait_warp(empty + 8 * (before % kStages), (before / kStages) & 1))) break;
+          const uint32_t at = base + kScales + step % kSlots * kSlotBytes;
           const float* rows = sa + static_cast<size_t>(b) * tokens;
 #pragma unroll
           for (int i = 0; i < kRows; i += 32) copy_scale(at + (i + lane) * 4, rows + min(row0 + i + lane, tokens - 1));
           if (lane < 2) copy_scale(at + (kRows + lane) * 4, weight + b);
-          copies_arrive(scaled + 8 * slot);
+          copies_arrive(rank == 0 ? full + 8 * (step % kStages) : scaled + 8 * (step % kSlots));
         }
       }
-      // (the arrival without copies that the adding warps ask about after the last block)
-      if (healthy && step >= kSlots) healthy = wait_warp(taken + 8 * (step % kSlots), (step / kSlots - 1) & 1);
-      if (healthy) copies_arrive(scaled + 8 * (step % kSlots));
       copies_wait();
+    } else if (rank == 1) {
+      // The peer's warp 1 tells the leader that the peer's scales are there.
+      const uint32_t leader_full = at_rank(full, 0);
+      const int steps = (tiles - pair + pairs - 1) / pairs * blocks;
+      for (int step = 0; warp == 1 && step < steps; ++step) {
+        if (!(healthy = wait_warp(scaled + 8 * (step % kSlots), (step / kSlots) & 1))) break;
+        if (lane == 0) arrive_remote(leader_full + 8 * (step % kStages));
+      }
+      // (both see the leader's empty commits arrive before the CTA ends)
+      const int buffer = (steps & 1) * 2 + (warp >> 1);
+      if (healthy) healthy = wait_warp(filled + 8 * buffer, (steps / 2) & 1);
     } else {
       // Two warps of the leader issue, one for each half of the outputs.  A warp's instructions wait in line behind its own products, so
       // one warp alone would test the next barriers only once its products are in the pipe, and the pipe would run dry
       // for the time of those tests.
       const int half = warp >> 1, steps = (tiles - pair + pairs - 1) / pairs * blocks;
       int step = 0;
-      for (; rank == 0 && step < steps; ++step) {
+      for (; step < steps; ++step) {
         const int s = step % kStages, buffer = (step & 1) * 2 + half;
         if (!(healthy = wait_warp(full + 8 * s, (step / kStages) & 1))) break;
         if (step >= 2 && !(healthy = wait_warp(drained + 8 * buffer, (step / 2 - 1) & 1))) break;
@@ -486,8 +496,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       // (No sooner than a product could come: one that overtook a warp still waiting for the block before would turn the
       // barrier's phase over twice.)
       const int buffer = (steps & 1) * 2 + half;
-      if (rank == 0 && healthy && steps >= 2) healthy = wait_warp(drained + 8 * buffer, (steps / 2 - 1) & 1);
-      if (rank == 0 && healthy && elect_one()) commit_pair(filled + 8 * buffer);
+      if (healthy && steps >= 2) healthy = wait_warp(drained + 8 * buffer, (steps / 2 - 1) & 1);
+      if (healthy && elect_one()) commit_pair(filled + 8 * buffer);
       __syncwarp();
       if (healthy) healthy = wait_warp(filled + 8 * buffer, (steps / 2) & 1);
       else if (step > 0) wait_warp(filled + 8 * (((step - 1) & 1) * 2 + half), ((step - 1) / 2) & 1);
@@ -495,12 +505,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * kHalf;
-    const uint32_t leader_drained = at_rank(drained, 0) + 8 * half;
-    const uint32_t row_scale = base + kScales + (quarter * 32 + lane) * 4, col_scale = base + kScales + (kRows + half) * 4;
+    // State of the block at hand, carried along because this loop is bound by its instructions: its accumulator, the
+    // barriers of that and their phase, its scales.  (Columns and barriers of the two parities differ in one bit.)
+    uint32_t columns = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * kHalf;
+    uint32_t ready = filled + 8 * half, free = at_rank(drained, 0) + 8 * half, phase = 0, scales = base + kScales;
+    auto next_block = [&] {
+      columns ^= 2 * kHalf;
+      ready ^= 16;
+      free ^= 16;
+      phase ^= (ready & 16) == 0 ? 1u : 0u;
+      scales = scales == base + kScales + (kSlots - 1) * kSlotBytes ? base + kScales : scales + kSlotBytes;
+    };
     uint8_t* store = shared + kStore + (warp - 4) * 2 * 32 * 128;
-    const uint32_t mine = filled + 8 * half;
-    int step = 0;
     for (int tile = pair; tile < tiles && healthy; tile += pairs) {
       float sum[kHalf];
 #pragma unroll
@@ -513,21 +529,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       // measured to cost a tenth of the kernel.)
       uint32_t d[2][32];
       float2 factors;
-      auto begin = [&](int at) {  // a block whose products and scales are there
+      auto begin = [&] {  // a block whose products are complete
         fence_after_sync();
-        load32(lane_base + (at & 1) * (2 * kHalf), d[0]);
-        factors = make_float2(load_shared(row_scale + at % kSlots * (kSlotFloats * 4)),
-                              load_shared(col_scale + at % kSlots * (kSlotFloats * 4)));
+        load32(columns, d[0]);
+        factors = make_float2(load_shared(scales + (quarter * 32 + lane) * 4), load_shared(scales + (kRows + half) * 4));
       };
       bool begun = false;
       for (int b = 0; b < blocks; ++b) {
         if (!begun) {
-          if (!(healthy = wait_warp(mine + 16 * (step & 1), (step / 2) & 1) &&
-                          wait_warp(scaled + 8 * (step % kSlots), (step / kSlots) & 1)))
-            break;
-          begin(step);
+          if (!(healthy = wait_warp(ready, phase))) break;
+          begin();
         }
-        const uint32_t columns = lane_base + (step & 1) * (2 * kHalf);
         const float scale = __fmul_rn(factors.x, factors.y);
         bool complete = false;
 #pragma unroll
@@ -535,21 +547,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           wait_loads(d[g & 1]);
           if (g + 1 < kHalf / 32) {
             load32(columns + (g + 1) * 32, d[(g + 1) & 1]);
-            if (g + 2 == kHalf / 32) {
-              const bool products = barrier_try(mine + 16 * (~step & 1), ((step + 1) / 2) & 1);
-              const bool scales = barrier_try(scaled + 8 * ((step + 1) % kSlots), ((step + 1) / kSlots) & 1);
-              complete = products & scales;
-            }
+            if (g + 2 == kHalf / 32) complete = barrier_try(ready ^ 16, phase ^ ((ready >> 4) & 1));
           } else {
             fence_before_sync();
             __syncwarp();
-            if (lane == 0) {
-              arrive_remote(leader_drained + 16 * (step & 1));
-              barrier_arrive(taken + 8 * (step % kSlots));
-            }
-            ++step;
+            if (lane == 0) arrive_remote(free);
+            next_block();
             begun = b + 1 < blocks && __all_sync(kFullMask, complete);
-            if (begun) begin(step);
+            if (begun) begin();
           }
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {

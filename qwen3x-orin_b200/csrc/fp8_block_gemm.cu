@@ -222,17 +222,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       }
-      // An empty commit where the next product would arrive, and no sooner: the adding warps ask about it after the last
-      // block, and a question about products that never come would hold them for microseconds.  It is complete when all
-      // products of this warp are, so that none of them reads shared memory any more.
-      if (healthy && step >= kBuffers) healthy = wait_warp(drained + 8 * (step % kBuffers), (step / kBuffers - 1) & 1);
-      if (healthy) {
-        if (elect_one()) commit(filled + 8 * (step % kBuffers));
-        __syncwarp();
-        healthy = wait_warp(filled + 8 * (step % kBuffers), (step / kBuffers) & 1);
-      } else if (step >= 2) {
-        wait_warp(filled + 8 * ((step - 2) % kBuffers), ((step - 2) / kBuffers) & 1);
-      }
+      // (products complete in order: after this warp's last one none of them is reading shared memory)
+      if (step >= 2 && !wait_warp(filled + 8 * ((step - 2) % kBuffers), ((step - 2) / kBuffers) & 1)) healthy = false;
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
@@ -245,39 +236,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       float sum[kMine];
 #pragma unroll
       for (int i = 0; i < kMine; ++i) sum[i] = 0.0f;
-      // One block: 32 columns of its accumulator at a time, times its scales, onto the sums; the next 32 columns, which may
-      // be the next block's first, are on their way meanwhile.
-      // Whether its products are complete is asked before the last columns but one are added and answered after.
-      uint32_t d[2][32];
-      float2 factors;
-      auto begin = [&](int at) {  // a block whose products are complete
+      for (int b = 0; b < blocks; ++b, ++step) {
+        if (!(healthy = wait_warp(filled + 8 * (step % kBuffers), (step / kBuffers) & 1))) break;
         fence_after_sync();
-        load32(lane_base + at % kBuffers * kCols, d[0]);
-        factors = make_float2(load_shared(row_scale + at % kSlots * (kSlotFloats * 4)),
-                              load_shared(col_scale + at % kSlots * (kSlotFloats * 4)));
-      };
-      bool begun = false;
-      for (int b = 0; b < blocks; ++b) {
-        if (!begun) {
-          if (!(healthy = wait_warp(filled + 8 * (step % kBuffers), (step / kBuffers) & 1))) break;
-          begin(step);
-        }
+        // the block's accumulator, 32 columns at a time and the next 32 on their way meanwhile, times its scales
         const uint32_t columns = lane_base + step % kBuffers * kCols;
-        const float scale = __fmul_rn(factors.x, factors.y);
-        bool complete = false;
+        uint32_t d[2][32];
+        load32(columns, d[0]);
+        const float scale = __fmul_rn(load_shared(row_scale + step % kSlots * (kSlotFloats * 4)),
+                                      load_shared(col_scale + step % kSlots * (kSlotFloats * 4)));
 #pragma unroll
         for (int g = 0; g < kMine / 32; ++g) {
           wait_loads(d[g & 1]);
           if (g + 1 < kMine / 32) {
             load32(columns + (g + 1) * 32, d[(g + 1) & 1]);
-            if (g + 2 == kMine / 32) complete = barrier_try(filled + 8 * ((step + 1) % kBuffers), ((step + 1) / kBuffers) & 1);
           } else {
             fence_before_sync();
             __syncwarp();
             if (lane == 0) barrier_arrive(drained + 8 * (step % kBuffers));
-            ++step;
-            begun = b + 1 < blocks && __all_sync(kFullMask, complete);
-            if (begun) begin(step);
           }
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
@@ -468,9 +444,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(healthy = wait_warp(scaled + 8 * (step % kSlots), (step / kSlots) & 1))) break;
         if (lane == 0) arrive_remote(leader_full + 8 * (step % kStages));
       }
-      // (both see the leader's empty commits arrive before the CTA ends)
-      const int buffer = (steps & 1) * 2 + (warp >> 1);
-      if (healthy) healthy = wait_warp(filled + 8 * buffer, (steps / 2) & 1);
     } else {
       // Two warps of the leader issue, one for each half of the outputs.  A warp's instructions wait in line behind its own products, so
       // one warp alone would test the next barriers only once its products are in the pipe, and the pipe would run dry
@@ -491,16 +464,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       }
-      // The empty commit; it is complete when all products of this warp are, so that none of them reads shared memory any
-      // more, and both CTAs see it arrive before they end.
-      // (No sooner than a product could come: one that overtook a warp still waiting for the block before would turn the
-      // barrier's phase over twice.)
-      const int buffer = (steps & 1) * 2 + half;
-      if (healthy && steps >= 2) healthy = wait_warp(drained + 8 * buffer, (steps / 2 - 1) & 1);
-      if (healthy && elect_one()) commit_pair(filled + 8 * buffer);
-      __syncwarp();
-      if (healthy) healthy = wait_warp(filled + 8 * buffer, (steps / 2) & 1);
-      else if (step > 0) wait_warp(filled + 8 * (((step - 1) & 1) * 2 + half), ((step - 1) / 2) & 1);
+      // (products complete in order: after this warp's last one none of them is reading shared memory)
+      if (step > 0 && !wait_warp(filled + 8 * (((step - 1) & 1) * 2 + half), ((step - 1) / 2) & 1)) healthy = false;
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
@@ -521,40 +486,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       float sum[kHalf];
 #pragma unroll
       for (int i = 0; i < kHalf; ++i) sum[i] = 0.0f;
-      // One block: 32 columns of its accumulator at a time, times its scales, onto the sums; the next 32 columns, which may
-      // be the next block's first, are on their way meanwhile.  Whether that block's products are complete is asked
-      // before the last columns but one are added and answered after.  (After the very last block the
-      // answer comes from an empty commit and an arrival without copies: a question about products that never come would
-      // hold the warp for microseconds, and asking only before other blocks, by a branch or by another barrier, was
-      // measured to cost a tenth of the kernel.)
-      uint32_t d[2][32];
-      float2 factors;
-      auto begin = [&] {  // a block whose products are complete
-        fence_after_sync();
-        load32(columns, d[0]);
-        factors = make_float2(load_shared(scales + (quarter * 32 + lane) * 4), load_shared(scales + (kRows + half) * 4));
-      };
-      bool begun = false;
       for (int b = 0; b < blocks; ++b) {
-        if (!begun) {
-          if (!(healthy = wait_warp(ready, phase))) break;
-          begin();
-        }
-        const float scale = __fmul_rn(factors.x, factors.y);
-        bool complete = false;
+        if (!(healthy = wait_warp(ready, phase))) break;
+        fence_after_sync();
+        // the block's accumulator, 32 columns at a time and the next 32 on their way meanwhile, times its scales
+        uint32_t d[2][32];
+        load32(columns, d[0]);
+        const float scale = __fmul_rn(load_shared(scales + (quarter * 32 + lane) * 4), load_shared(scales + (kRows + half) * 4));
 #pragma unroll
         for (int g = 0; g < kHalf / 32; ++g) {
           wait_loads(d[g & 1]);
           if (g + 1 < kHalf / 32) {
             load32(columns + (g + 1) * 32, d[(g + 1) & 1]);
-            if (g + 2 == kHalf / 32) complete = barrier_try(ready ^ 16, phase ^ ((ready >> 4) & 1));
           } else {
             fence_before_sync();
             __syncwarp();
             if (lane == 0) arrive_remote(free);
             next_block();
-            begun = b + 1 < blocks && __all_sync(kFullMask, complete);
-            if (begun) begin();
           }
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {

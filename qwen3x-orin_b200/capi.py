@@ -137,21 +137,23 @@ def ptr(x):
 
 
 _functions = {}  # name -> bound entry point
-_addressed = {int: False, float: False, type(None): False}  # argument type -> whether it has a device address
+_addressed = {int: False, float: False, type(None): False}  # argument types: whether their values have a device address
 
 
 def call(name: str, *args) -> int:
     """Calls an entry point; tensor-likes are replaced by their device address.  (A batch-one call is bound by what
-    happens here, so an entry point is looked up and an argument type asked once.)"""
+    happens here, so an entry point is looked up once and a type that offers data_ptr() asked once.)"""
     fn = _functions.get(name)
     if fn is None:
         fn = _functions[name] = getattr(lib(), name)
     try:
-        return fn(*[a.data_ptr() if _addressed[a.__class__] else a for a in args])
-    except KeyError:  # a type not seen before
+        values = [a.data_ptr() if _addressed[a.__class__] else a for a in args]
+    except KeyError:  # a type not seen before, or one whose objects have to be asked one by one
         for a in args:
-            _addressed.setdefault(a.__class__, hasattr(a, "data_ptr"))
-    return fn(*[a.data_ptr() if _addressed[a.__class__] else a for a in args])
+            if hasattr(a.__class__, "data_ptr"):
+                _addressed.setdefault(a.__class__, True)
+        values = [a.data_ptr() if hasattr(a, "data_ptr") else a for a in args]
+    return fn(*values)
 
 
 def check(name: str, *args) -> None:

@@ -4,13 +4,16 @@
 // are summed in FP32 by the tensor cores, multiplied by the two scales and added to the running FP32 sum; the one rounding
 // is to bf16.
 //
-// Two kernels on tcgen05 (kind::f8f6f4: E4M3 x E4M3 -> FP32 in tensor memory), operands fetched by bulk tensor copies
+// Three kernels on tcgen05 (kind::f8f6f4: E4M3 x E4M3 -> FP32 in tensor memory), operands fetched by bulk tensor copies
 // into rings of 128-byte-swizzled stages, one stage per block of 128 columns of K:
-//   * panel: 128 tokens are the MMA's rows, 256 (or 128) outputs its columns; bound by the tensor cores;
-//   * strip: 128 outputs are the rows, 16 to 128 tokens the columns; bound by reading the weights.
+//   * strip: 128 outputs are the MMA's rows, 16 to 128 tokens its columns, K is split over a cluster; for few tokens,
+//     bound by reading the weights;
+//   * panel: 128 tokens are the rows, 128 outputs the columns, one CTA per tile; bound by how evenly the tiles fill the SMs;
+//   * pair:  256 tokens x 256 outputs on two SMs at once; for many tokens, bound by the tensor cores and their power.
 // The hardware's accumulator cannot be scaled between two blocks of K, so every block starts a fresh accumulator and the
-// scaled sum lives in registers: two accumulators alternate, and while the tensor cores fill one, the epilogue warps read
-// the other and add it, times its scale, to their FP32 sums.
+// scaled sum lives in registers: accumulators take turns, and while the tensor cores fill the others, the adding warps read
+// one and add it, times its scales, to their FP32 sums.  (A thread's sums stay with one warp for the whole of K: no order of
+// additions depends on timing.)
 //
 // Waits are bounded; one that runs out raises a sticky word (q3x_b200_fp8_block_gemm_error), and the CTA drains its
 // copies, frees its tensor memory and returns.
@@ -53,8 +56,8 @@ __device__ __forceinline__ void arrive_remote(uint32_t there) {
 }
 // Four floats into another CTA's shared memory; their bytes complete on a barrier of that CTA.
 __device__ __forceinline__ void push(uint32_t there, const float4& v, uint32_t barrier_there) {
-  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(there), "f"(v.x),
-               "f"(v.y), "f"(v.z), "f"(v.w), "r"(barrier_there)
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(there),
+               "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(barrier_there)
                : "memory");
 }
 __device__ __forceinline__ float4 add4(const float4& a, const float4& b) {
@@ -90,7 +93,10 @@ __device__ __forceinline__ uint32_t shared_address(const void* p) { return stati
 namespace panel {
 
 // Tiles of 128 tokens x 128 outputs, one CTA each: for products with too few tiles of 256 x 256 to give every pair of SMs
-// one.
+// one.  A block's product takes 256 cycles of the tensor cores, reading it and adding it up about as long, so that four
+// accumulators keep both busy.  512 x 10240 x 5120: 37.9 us, 1.42 PFLOP/s (160 tiles for 148 SMs, two rounds; pairs 41);
+// with all SMs even, 4096 x 10240 x 5120, the tensor pipe is active for 51 % of the time (pairs: 75 %), which is why pairs
+// take over as soon as they fill the GPU.
 constexpr int kRows = 128;                  // tokens of a tile
 constexpr int kCols = 128;                  // outputs of a tile
 constexpr int kThreads = 384;               // warp 0 fetches codes, 2 scales, 1 and 3 issue, 4 to 11 add up
@@ -117,7 +123,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                             int blocks, int row_tiles, int col_tiles, uint16_t* __restrict__ out) {
   extern __shared__ __align__(1024) uint8_t shared[];
   const uint32_t base = shared_address(shared);
-  const uint32_t full = base + kBarriers, empty = full + 8 * kStages, filled = empty + 8 * kStages, drained = filled + 8 * kBuffers;
+  const uint32_t full = base + kBarriers, empty = full + 8 * kStages, filled = empty + 8 * kStages,
+                 drained = filled + 8 * kBuffers;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(shared + kTmemSlot);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles = row_tiles * col_tiles;
@@ -309,7 +316,8 @@ namespace pair {
 // weights' codes, and one tensor instruction runs on both SMs (cta_group::2).  Against two tiles of 128 x 256 every SM
 // fetches 32 KB instead of 48 KB per block of K, and an instruction of 128 columns reads 6 KB of shared memory instead
 // of 8 in its 64 cycles, which is what lets the accumulators be four of 128 columns: each half of the outputs has two, and
-// a half is read while three other products run.
+// a half is read while three other products run.  8192 x 34816 x 5120: 1.04 to 1.12 ms from a cool start (2.6 to 2.8 PFLOP/s
+// of the 3.3 that twice the measured bf16 rate makes), 1.2 to 1.4 ms when the GPU holds its clocks down for power.
 constexpr int kRows = 128;                  // tokens of a CTA
 constexpr int kCols = 256;                  // outputs of a tile
 constexpr int kHalf = 128;                  // outputs of one product
@@ -445,9 +453,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) arrive_remote(leader_full + 8 * (step % kStages));
       }
     } else {
-      // Two warps of the leader issue, one for each half of the outputs.  A warp's instructions wait in line behind its own products, so
-      // one warp alone would test the next barriers only once its products are in the pipe, and the pipe would run dry
-      // for the time of those tests.
+      // Two warps of the leader issue, one for each half of the outputs.  A warp's instructions wait in line behind its own
+      // products, so one warp alone would test the next barriers only once its products are in the pipe, and the pipe would
+      // run dry for the time of those tests.
       const int half = warp >> 1, steps = (tiles - pair + pairs - 1) / pairs * blocks;
       int step = 0;
       for (; step < steps; ++step) {
@@ -557,6 +565,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ------------------------------------------------------------------------------------------------------------- strip
 namespace strip {
 
+// Outputs are the rows of the product, so that one token costs 16 columns and not a tile of 128 rows.  All that counts is to
+// keep the weights coming: 131 to 202 KB of them are in flight per SM, and K is split until every SM has a share.  One token,
+// 34816 x 5120: 30.1 us, 5.9 TB/s (0.90 of what a copy reaches); 5120 x 17408: 17.0 us (0.80); 48 tokens: 19.4 us.  What is left
+// is the fixed part, some 3 us of launch, first fetch and joining of sums, and the SMs that clusters of this size leave idle.
 constexpr int kRows = 128;     // outputs of a tile
 constexpr int kMaxSplits = 8;  // CTAs of a cluster, one share of K each
 
@@ -582,8 +594,8 @@ struct Shape {
 };
 
 // The cluster's CTAs share the blocks of K of one tile.  The sums of tokens 4 g to 4 g + 3 belong to rank g % splits:
-// everybody pushes them into that CTA's shared memory, the pushes complete on its barrier, and it adds them in rank order.  (Sums left in place and
-// read by the others took two fences at cluster scope for each tile, a microsecond each.)
+// everybody pushes them into that CTA's shared memory, the pushes complete on its barrier, and it adds them in rank order.
+// (Sums left in place and read by the others took two fences at cluster scope for each tile, a microsecond each.)
 template <int COLS>
 __global__ void __launch_bounds__(Shape<COLS>::kThreads, 1)
     block_gemm_strip_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
@@ -618,7 +630,8 @@ __global__ void __launch_bounds__(Shape<COLS>::kThreads, 1)
     barrier_init_fence();
   }
   if (warp == 2) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(const_cast<uint32_t*>(tmem_slot))),
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     shared_address(const_cast<uint32_t*>(tmem_slot))),
                  "r"(S::kColumns)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -722,7 +735,8 @@ __global__ void __launch_bounds__(Shape<COLS>::kThreads, 1)
           }
 #pragma unroll
           for (int i = 0; i < kGroup; i += 2) {
-            const float2 scale = mul2(i % 4 == 0 ? make_float2(f[i / 4].x, f[i / 4].y) : make_float2(f[i / 4].z, f[i / 4].w), weight);
+            const float2 scale =
+                mul2(i % 4 == 0 ? make_float2(f[i / 4].x, f[i / 4].y) : make_float2(f[i / 4].z, f[i / 4].w), weight);
             const float2 r = fma2(scale, make_float2(__uint_as_float(d[i]), __uint_as_float(d[i + 1])),
                                   make_float2(sum[g + i], sum[g + i + 1]));
             sum[g + i] = r.x;
@@ -743,8 +757,8 @@ __global__ void __launch_bounds__(Shape<COLS>::kThreads, 1)
 #pragma unroll
       for (int i = 0; i < kMine; i += 4) {
         if (col0 + i < visible)
-          push(at_rank(base + S::kPartial + (place * kRows + row) * 16, owner), make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]),
-               at_rank(ready, owner));
+          push(at_rank(base + S::kPartial + (place * kRows + row) * 16, owner),
+               make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]), at_rank(ready, owner));
         if (++owner == splits) {
           owner = 0;
           ++place;
@@ -855,15 +869,17 @@ int launch_panel(const Problem& p) {
   if (!encode_codes(&a, p.activations, p.tokens, p.in_features, panel::kRows) ||
       !encode_codes(&w, p.weights, p.out_features, p.in_features, panel::kCols))
     return host::kNotSupported;
-  const int row_tiles = (p.tokens + panel::kRows - 1) / panel::kRows, col_tiles = (p.out_features + panel::kCols - 1) / panel::kCols;
+  const int row_tiles = (p.tokens + panel::kRows - 1) / panel::kRows;
+  const int col_tiles = (p.out_features + panel::kCols - 1) / panel::kCols;
   const int tiles = row_tiles * col_tiles, sms = host::current_device_sm_count();
   host::launch_kernel(kernel, dim3(tiles < sms ? tiles : sms), dim3(panel::kThreads), panel::kShared, p.stream, true, a, w,
                       p.activation_scales, p.weight_scales, p.tokens, p.out_features, p.blocks, row_tiles, col_tiles, p.out);
   return host::launch_status();
 }
 
-// Clusters of `splits` CTAs of a prepared kernel that are resident at once (one CTA per SM; a cluster lives inside one group of SMs, so that
-// sizes that do not divide the groups leave SMs idle: 74 of two, 45 of three, 33 of four, 15 of seven or eight).
+// Clusters of `splits` CTAs of a prepared kernel that are resident at once (one CTA per SM; a cluster lives inside one
+// group of SMs, so that sizes that do not divide the groups leave SMs idle: 74 of two, 45 of three, 33 of four, 26 of five,
+// 22 of six, 15 of seven or eight).
 template <auto kKernel, int kThreads>
 int resident_clusters(int splits, int shared) {
   constexpr int kMaxDevices = 64;
@@ -919,7 +935,8 @@ int launch_pair(const Problem& p) {
       !encode_codes(&w, p.weights, p.out_features, p.in_features, pair::kHalf / 2) ||
       !encode_map(&o, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.out, p.tokens, p.out_features, 32))
     return host::kNotSupported;
-  const int row_tiles = (p.tokens + 2 * pair::kRows - 1) / (2 * pair::kRows), col_tiles = (p.out_features + pair::kCols - 1) / pair::kCols;
+  const int row_tiles = (p.tokens + 2 * pair::kRows - 1) / (2 * pair::kRows);
+  const int col_tiles = (p.out_features + pair::kCols - 1) / pair::kCols;
   const int tiles = row_tiles * col_tiles, resident = resident_clusters<kernel, pair::kThreads>(2, pair::kShared);
   return launch_clusters<kernel>(p, 2, tiles < resident ? tiles : resident, pair::kThreads, pair::kShared, a, w, o,
                                  p.activation_scales, p.weight_scales, p.tokens, p.out_features, p.blocks, row_tiles, col_tiles);
@@ -968,7 +985,9 @@ int launch_strip(const Problem& p) {
 // of 128 tokens 3.6 + 0.48 us and 3.5 us for the sums of a tile (128 x 5120 x 5120: 13.9 us, panels 14.4, pairs 20.0).
 int launch_many(const Problem& p) {
   const long long sms = host::current_device_sm_count(), pairs = sms / 2 > 0 ? sms / 2 : 1;
-  auto tiles = [&](long long rows, long long cols) { return (p.tokens + rows - 1) / rows * ((p.out_features + cols - 1) / cols); };
+  auto tiles = [&](long long rows, long long cols) {
+    return (p.tokens + rows - 1) / rows * ((p.out_features + cols - 1) / cols);
+  };
   const long long panel_time = 300 + (tiles(panel::kRows, panel::kCols) + sms - 1) / sms * p.blocks * 28;
   const long long pair_time = 450 + (tiles(2 * pair::kRows, pair::kCols) + pairs - 1) / pairs * p.blocks * 40;
   if (p.tokens <= 128) {

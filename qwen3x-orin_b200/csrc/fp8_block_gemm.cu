@@ -9,7 +9,7 @@
 //   * strip: 128 outputs are the MMA's rows, 16 to 128 tokens its columns, K is split over a cluster; for few tokens,
 //     bound by reading the weights;
 //   * panel: 128 tokens are the rows, 128 outputs the columns, one CTA per tile; bound by how evenly the tiles fill the SMs;
-//   * pair:  256 tokens x 256 outputs on two SMs at once; for many tokens, bound by the tensor cores and their power.
+//   * pair:  256 tokens x 256 (or 160) outputs on two SMs at once; for many tokens, bound by the tensor cores and their power.
 // The hardware's accumulator cannot be scaled between two blocks of K, so every block starts a fresh accumulator and the
 // scaled sum lives in registers: accumulators take turns, and while the tensor cores fill the others, the adding warps read
 // one and add it, times its scales, to their FP32 sums.  (A thread's sums stay with one warp for the whole of K: no order of
@@ -93,10 +93,9 @@ __device__ __forceinline__ uint32_t shared_address(const void* p) { return stati
 namespace panel {
 
 // Tiles of 128 tokens x 128 outputs, one CTA each: for products with too few tiles of 256 x 256 to give every pair of SMs
-// one.  A block's product takes 256 cycles of the tensor cores, reading it and adding it up about as long, so that four
-// accumulators keep both busy.  512 x 10240 x 5120: 37.9 us, 1.42 PFLOP/s (160 tiles for 148 SMs, two rounds; pairs 41);
-// with all SMs even, 4096 x 10240 x 5120, the tensor pipe is active for 51 % of the time (pairs: 75 %), which is why pairs
-// take over as soon as they fill the GPU.
+// one.  A block's product takes 256 cycles of the tensor cores, but its 32 KB come at 64 bytes per cycle at most, in 512:
+// that bounds it (4096 x 10240 x 5120: 65 bytes per cycle and SM leave L2, the tensor pipe is active for 51 % of the time), and
+// is why pairs take over as soon as they fill the GPU.  200 x 5120 x 17408: 41.7 us (pairs 46.2), 777 x 5120 x 6144: 35.4 us (38.7).
 constexpr int kRows = 128;                  // tokens of a tile
 constexpr int kCols = 128;                  // outputs of a tile
 constexpr int kThreads = 384;               // warp 0 fetches codes, 2 scales, 1 and 3 issue, 4 to 11 add up
@@ -316,39 +315,66 @@ namespace pair {
 // weights' codes, and one tensor instruction runs on both SMs (cta_group::2).  Against two tiles of 128 x 256 every SM
 // fetches 32 KB instead of 48 KB per block of K, and an instruction of 128 columns reads 6 KB of shared memory instead
 // of 8 in its 64 cycles, which is what lets the accumulators be four of 128 columns: each half of the outputs has two, and
-// a half is read while three other products run.  8192 x 34816 x 5120: 1.04 to 1.12 ms from a cool start (2.6 to 2.8 PFLOP/s
+// a half is read while three other products run.  8192 x 34816 x 5120: 1.01 to 1.13 ms from a cool start (2.6 to 2.9 PFLOP/s
 // of the 3.3 that twice the measured bf16 rate makes), 1.2 to 1.4 ms when the GPU holds its clocks down for power.
+//
+// Tiles of 256 tokens x 160 outputs are for products whose tiles of 256 x 256 would leave many SMs idle in their last (or
+// only) round.  Their block is one product of all outputs, with three accumulators; their border between two weight blocks
+// can lie anywhere.  256 x 10240 x 5120: 17.4 us (256 outputs 20.4, panels 25.9), 512 x 10240 x 5120: 30.2 us (33.5, 39).
+// A block takes 0.31 us with few SMs at work; with the additions left out 0.24, with three of four products left out too the
+// same: fetching it, 26 KB per SM at 64 bytes per cycle, is the bound.  (Tiles of 96 or 128 outputs: 0.28 us.)
 constexpr int kRows = 128;                  // tokens of a CTA
-constexpr int kCols = 256;                  // outputs of a tile
-constexpr int kHalf = 128;                  // outputs of one product
 constexpr int kThreads = 384;               // warp 0 fetches codes, 2 scales, 1 and 3 issue (leader), 4 to 11 add up
-constexpr int kAdders = 8;                  // warps: 4 lane quarters x 2 halves
+constexpr int kAdders = 8;                  // warps: 4 lane quarters x 2 halves of the outputs
 constexpr int kLaunchRegisters = 168;       // 65536 / 384, rounded down to 8
 constexpr int kBand = 8;                    // token tiles walked together
-constexpr int kBuffers = 4;                 // accumulators: parity of the block x half
-constexpr int kStageBytes = (kRows + kCols / 2) * kRowBytes;
-constexpr int kStages = 5;
-constexpr int kSlots = 5;                   // of scales
-constexpr int kSlotBytes = (kRows + 2) * 4;  // the tokens', the two halves' weight blocks'
-constexpr int kAhead = 3;                   // blocks that scales are fetched before their products
-static_assert(kSlots >= kAhead + 2, "see the warp that fetches scales");
-constexpr int kStore = kStages * kStageBytes;                  // [adder][2][32 rows][64 outputs] bf16
-constexpr int kScales = kStore + kAdders * 2 * 32 * 128;
-constexpr int kBarriers = (kScales + kSlots * kSlotBytes + 31) / 32 * 32;  // (the accumulators' come first: see next_block)
-constexpr int kTmemSlot = kBarriers + 8 * (2 * kStages + 2 * kBuffers + kSlots);
-constexpr int kShared = kTmemSlot + 16;
-static_assert(kShared <= 232448, "shared memory of one CTA");
+constexpr int kMostShared = 232448;         // shared memory of one CTA
 
+template <int COLS>  // outputs of a tile
+struct Shape {
+  static constexpr int kProducts = COLS == 256 ? 2 : 1;          // per block; each has a range of the outputs
+  static constexpr int kWide = COLS / kProducts;                 // outputs of a product
+  static constexpr int kDepth = 512 / COLS;                      // accumulators per range of outputs
+  static constexpr int kBuffers = kProducts * kDepth;
+  static constexpr int kMine = COLS / 2;                         // outputs of one adding warp
+  static constexpr int kBox = kMine % 64 == 0 ? 64 : 16;   // outputs of one store
+  static constexpr bool kAligned = 128 % kMine == 0;             // a warp's outputs lie in one weight block
+  static constexpr int kStageBytes = (kRows + COLS / 2) * kRowBytes;
+  static constexpr int kSlots = COLS == 256 ? 5 : 7;             // of scales, one per block in flight
+  static constexpr int kSlotBytes = (kRows + 4) * 4;             // the tokens', two weight blocks' for each half of the outputs
+  static constexpr int kStoreBytes = kAdders * 32 * kMine * 2;   // [adder][box][32 rows][kBox outputs] bf16
+  static constexpr int kStages = (kMostShared - kStoreBytes - kSlots * kSlotBytes - 384) / kStageBytes;
+  static constexpr int kStore = kStages * kStageBytes;
+  static constexpr int kScales = kStore + kStoreBytes;
+  static constexpr int kBarriers = (kScales + kSlots * kSlotBytes + 31) / 32 * 32;  // (accumulators' first: see next_block)
+  static constexpr int kTmemSlot = kBarriers + 8 * (2 * kStages + 2 * kBuffers + 2 * kSlots);
+  static constexpr int kShared = kTmemSlot + 16;
+  static_assert(COLS % 32 == 0 && kMine % kBox == 0 && kWide <= 256 && kBuffers * kWide <= 512 && kStageBytes % 1024 == 0);
+  static_assert(kShared <= kMostShared);
+  // (scales arrive on their stage's barrier: those of a block must not come before the stage's last block was complete)
+  static_assert(kSlots <= kStages);
+};
+
+// Columns first to first + 31 of an adding warp's kMine (or the 16 that are left) into registers.
+template <int kMine>
+__device__ __forceinline__ void load_columns(uint32_t columns, int first, uint32_t (&d)[32]) {
+  if (kMine % 32 == 0 || first + 32 <= kMine) load32(columns + first, d);
+  else load16(columns + first, reinterpret_cast<uint32_t (&)[16]>(d));
+}
+
+template <int COLS>
 __global__ void __launch_bounds__(kThreads, 1)
     block_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                            const __grid_constant__ CUtensorMap map_out, const float* __restrict__ sa,
                            const float* __restrict__ sw, int tokens, int out_features, int blocks, int row_tiles,
                            int col_tiles) {
+  using S = Shape<COLS>;
+  constexpr int kStages = S::kStages, kBuffers = S::kBuffers, kSlots = S::kSlots, kProducts = S::kProducts, kWide = S::kWide;
   extern __shared__ __align__(1024) uint8_t shared[];
   const uint32_t base = shared_address(shared);
-  const uint32_t filled = base + kBarriers, drained = filled + 8 * kBuffers, full = drained + 8 * kBuffers,
-                 empty = full + 8 * kStages, scaled = empty + 8 * kStages;
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(shared + kTmemSlot);
+  const uint32_t filled = base + S::kBarriers, drained = filled + 8 * kBuffers, full = drained + 8 * kBuffers,
+                 empty = full + 8 * kStages, scaled = empty + 8 * kStages, taken = scaled + 8 * kSlots;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(shared + S::kTmemSlot);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, tiles = row_tiles * col_tiles;
 
@@ -359,17 +385,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < kStages; ++s) {
       // (the leader's: both CTAs' codes complete on it; its own scales' lanes arrive, and the peer's warp 1 for its scales)
       barrier_init(full + 8 * s, 1 + 32 + 1);
-      barrier_init(empty + 8 * s, 2);   // both halves' products
+      barrier_init(empty + 8 * s, kProducts);
     }
     for (int i = 0; i < kBuffers; ++i) {
       barrier_init(filled + 8 * i, 1);
-      barrier_init(drained + 8 * i, kAdders);  // (the leader's: four warps of each CTA)
+      barrier_init(drained + 8 * i, 2 * kAdders / kProducts);  // (the leader's: the warps of both CTAs that read it)
     }
-    for (int i = 0; i < kSlots; ++i) barrier_init(scaled + 8 * i, 32);
+    for (int i = 0; i < kSlots; ++i) {
+      barrier_init(scaled + 8 * i, 32);
+      barrier_init(taken + 8 * i, kAdders);
+    }
     barrier_init_fence();
   }
   if (warp == 2) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + kTmemSlot), "r"(kBuffers * kHalf)
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + S::kTmemSlot), "r"(512)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
@@ -401,16 +430,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int tile = pair; tile < tiles && healthy; tile += pairs) {
         int row_tile, col_tile;
         tile_at(tile, row_tile, col_tile);
-        const int row0 = (row_tile * 2 + rank) * kRows, col0 = col_tile * kCols + rank * (kHalf / 2);
+        const int row0 = (row_tile * 2 + rank) * kRows, col0 = col_tile * COLS + rank * (kWide / 2);
         for (int b = 0; b < blocks; ++b, ++step) {
           const int s = step % kStages;
           if (step >= kStages && !(healthy = wait_warp(empty + 8 * s, (step / kStages - 1) & 1))) break;
-          const uint32_t at = base + s * kStageBytes;
+          const uint32_t at = base + s * S::kStageBytes;
           if (elect_one()) {
-            if (rank == 0) barrier_expect(full + 8 * s, 2 * kStageBytes);
+            if (rank == 0) barrier_expect(full + 8 * s, 2 * S::kStageBytes);
             load_box_pair(at, &map_a, b * kBlockK, row0, leader_full + 8 * s);
-            load_box_pair(at + kRows * kRowBytes, &map_w, b * kBlockK, col0, leader_full + 8 * s);
-            load_box_pair(at + (kRows + kHalf / 2) * kRowBytes, &map_w, b * kBlockK, col0 + kHalf, leader_full + 8 * s);
+#pragma unroll
+            for (int i = 0; i < kProducts; ++i)
+              load_box_pair(at + (kRows + i * (kWide / 2)) * kRowBytes, &map_w, b * kBlockK, col0 + i * kWide, leader_full + 8 * s);
           }
         }
       }
@@ -422,8 +452,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 2) {
       // The scales of a block, copied without passing through registers (a load held in one for two blocks was measured to
       // hold up the whole warp wherever the compiler moved it).  Products wait for them, so that the adding warps need not.
-      // A slot is free again: when step t - kAhead has left its stage, its accumulators had come round, so step
-      // t - kAhead - 2 was drained and its scales read; slot t % kSlots holds a step at least that old.
+      // A slot is free again when this CTA's adding warps have read it.  (Asking instead for the product that must have
+      // followed that came two blocks later, and three blocks ahead left 690 cycles per block, whatever the tile.)
       const int weight_rows = (out_features + kBlockK - 1) / kBlockK;
       int step = 0;
       for (int tile = pair; tile < tiles && healthy; tile += pairs) {
@@ -431,16 +461,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         tile_at(tile, row_tile, col_tile);
         // (a token or weight block past the end takes the last one's scale: its sums are not stored)
         const int row0 = (row_tile * 2 + rank) * kRows;
-        const float* weight = sw + static_cast<size_t>(min(col_tile * 2 + (lane & 1), weight_rows - 1)) * blocks;
+        const int weight_row = (col_tile * COLS + (lane >> 1 & 1) * S::kMine) / kBlockK + (lane & 1);
+        const float* weight = sw + static_cast<size_t>(min(weight_row, weight_rows - 1)) * blocks;
         for (int b = 0; b < blocks; ++b, ++step) {
-          const int before = step - kAhead;
-          if (before >= 0 && !(healthy = wait_warp(empty + 8 * (before % kStages), (before / kStages) & 1))) break;
-          const uint32_t at = base + kScales + step % kSlots * kSlotBytes;
+          const int slot = step % kSlots;
+          if (step >= kSlots && !(healthy = wait_warp(taken + 8 * slot, (step / kSlots - 1) & 1))) break;
+          const uint32_t at = base + S::kScales + slot * S::kSlotBytes;
           const float* rows = sa + static_cast<size_t>(b) * tokens;
 #pragma unroll
           for (int i = 0; i < kRows; i += 32) copy_scale(at + (i + lane) * 4, rows + min(row0 + i + lane, tokens - 1));
-          if (lane < 2) copy_scale(at + (kRows + lane) * 4, weight + b);
-          copies_arrive(rank == 0 ? full + 8 * (step % kStages) : scaled + 8 * (step % kSlots));
+          if (lane < 4) copy_scale(at + (kRows + lane) * 4, weight + b);
+          copies_arrive(rank == 0 ? full + 8 * (step % kStages) : scaled + 8 * slot);
         }
       }
       copies_wait();
@@ -453,95 +484,118 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) arrive_remote(leader_full + 8 * (step % kStages));
       }
     } else {
-      // Two warps of the leader issue, one for each half of the outputs.  A warp's instructions wait in line behind its own
-      // products, so one warp alone would test the next barriers only once its products are in the pipe, and the pipe would
-      // run dry for the time of those tests.
-      const int half = warp >> 1, steps = (tiles - pair + pairs - 1) / pairs * blocks;
-      int step = 0;
-      for (; step < steps; ++step) {
-        const int s = step % kStages, buffer = (step & 1) * 2 + half;
+      // Two warps of the leader issue, a product each in turn.  A warp's instructions wait in line behind its own products, so
+      // one warp alone would test the next barriers only once its products are in the pipe, and the pipe would run dry
+      // for the time of those tests.
+      const int products = (tiles - pair + pairs - 1) / pairs * blocks * kProducts;
+      int product = warp >> 1;
+      for (; product < products; product += 2) {
+        const int step = product / kProducts, s = step % kStages, buffer = product % kBuffers, round = product / kBuffers;
         if (!(healthy = wait_warp(full + 8 * s, (step / kStages) & 1))) break;
-        if (step >= 2 && !(healthy = wait_warp(drained + 8 * buffer, (step / 2 - 1) & 1))) break;
+        if (round > 0 && !(healthy = wait_warp(drained + 8 * buffer, (round - 1) & 1))) break;
         fence_after_sync();
-        const uint32_t at = base + s * kStageBytes;
+        const uint32_t at = base + s * S::kStageBytes;
         if (elect_one()) {
-          block_product_pair(tmem + buffer * kHalf, at, at + (kRows + half * (kHalf / 2)) * kRowBytes,
-                             instruction_descriptor_e4m3(kHalf, 256));
+          block_product_pair(tmem + buffer * kWide, at, at + (kRows + product % kProducts * (kWide / 2)) * kRowBytes,
+                             instruction_descriptor_e4m3(kWide, 256));
           commit_pair(filled + 8 * buffer);
           commit_pair(empty + 8 * s);
         }
         __syncwarp();
       }
       // (products complete in order: after this warp's last one none of them is reading shared memory)
-      if (step > 0 && !wait_warp(filled + 8 * (((step - 1) & 1) * 2 + half), ((step - 1) / 2) & 1)) healthy = false;
+      const int last = product - 2;
+      if (last >= 0 && !wait_warp(filled + 8 * (last % kBuffers), (last / kBuffers) & 1)) healthy = false;
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     // State of the block at hand, carried along because this loop is bound by its instructions: its accumulator, the
-    // barriers of that and their phase, its scales.  (Columns and barriers of the two parities differ in one bit.)
-    uint32_t columns = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * kHalf;
-    uint32_t ready = filled + 8 * half, free = at_rank(drained, 0) + 8 * half, phase = 0, scales = base + kScales;
+    // barriers of that and their phase, its scales.  (With two accumulators per half, columns and barriers differ in one bit.)
+    const int mine = kProducts == 2 ? half * kWide : half * S::kMine, own = kProducts == 2 ? half : 0;
+    uint32_t columns = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + mine;
+    uint32_t ready = filled + 8 * own, free = at_rank(drained, 0) + 8 * own, phase = 0, scales = base + S::kScales, read = taken;
     auto next_block = [&] {
-      columns ^= 2 * kHalf;
-      ready ^= 16;
-      free ^= 16;
-      phase ^= (ready & 16) == 0 ? 1u : 0u;
-      scales = scales == base + kScales + (kSlots - 1) * kSlotBytes ? base + kScales : scales + kSlotBytes;
+      if constexpr (kProducts == 2) {
+        columns ^= 2 * kWide;
+        ready ^= 16;
+        free ^= 16;
+        phase ^= (ready & 16) == 0 ? 1u : 0u;
+      } else {
+        const bool last = ready == filled + 8 * (kBuffers - 1);
+        columns = last ? columns - (kBuffers - 1) * kWide : columns + kWide;
+        ready = last ? filled : ready + 8;
+        free = last ? free - 8 * (kBuffers - 1) : free + 8;
+        phase ^= last ? 1u : 0u;
+      }
+      const bool last = read == taken + 8 * (kSlots - 1);
+      scales = last ? base + S::kScales : scales + S::kSlotBytes;
+      read = last ? taken : read + 8;
     };
-    uint8_t* store = shared + kStore + (warp - 4) * 2 * 32 * 128;
+    constexpr int kMine = S::kMine, kBoxBytes = 32 * S::kBox * 2, kPieces = S::kBox / 8;
+    uint8_t* store = shared + S::kStore + (warp - 4) * (kMine / S::kBox) * kBoxBytes;
     for (int tile = pair; tile < tiles && healthy; tile += pairs) {
-      float sum[kHalf];
+      float sum[kMine];
 #pragma unroll
-      for (int i = 0; i < kHalf; ++i) sum[i] = 0.0f;
+      for (int i = 0; i < kMine; ++i) sum[i] = 0.0f;
+      int row_tile, col_tile;
+      tile_at(tile, row_tile, col_tile);
+      const int x = col_tile * COLS + half * kMine, y = (row_tile * 2 + rank) * kRows + quarter * 32;
+      const int border = kBlockK - x % kBlockK;  // this warp's outputs before it lie in one weight block, the others in the next
       for (int b = 0; b < blocks; ++b) {
         if (!(healthy = wait_warp(ready, phase))) break;
         fence_after_sync();
         // the block's accumulator, 32 columns at a time and the next 32 on their way meanwhile, times its scales
         uint32_t d[2][32];
-        load32(columns, d[0]);
-        const float scale = __fmul_rn(load_shared(scales + (quarter * 32 + lane) * 4), load_shared(scales + (kRows + half) * 4));
+        load_columns<kMine>(columns, 0, d[0]);
+        const float row_scale = load_shared(scales + (quarter * 32 + lane) * 4);
+        const float scale = __fmul_rn(row_scale, load_shared(scales + (kRows + half * 2) * 4));
+        const float scale_beyond = S::kAligned ? scale : __fmul_rn(row_scale, load_shared(scales + (kRows + half * 2 + 1) * 4));
 #pragma unroll
-        for (int g = 0; g < kHalf / 32; ++g) {
-          wait_loads(d[g & 1]);
-          if (g + 1 < kHalf / 32) {
-            load32(columns + (g + 1) * 32, d[(g + 1) & 1]);
+        for (int g = 0; g < kMine; g += 32) {
+          wait_loads(d[g / 32 & 1]);
+          if (g + 32 < kMine) {
+            load_columns<kMine>(columns, g + 32, d[(g / 32 + 1) & 1]);
           } else {
             fence_before_sync();
             __syncwarp();
-            if (lane == 0) arrive_remote(free);
+            if (lane == 0) {
+              arrive_remote(free);
+              barrier_arrive(read);
+            }
             next_block();
           }
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float2 r = fma2(make_float2(scale, scale),
-                                  make_float2(__uint_as_float(d[g & 1][i]), __uint_as_float(d[g & 1][i + 1])),
-                                  make_float2(sum[g * 32 + i], sum[g * 32 + i + 1]));
-            sum[g * 32 + i] = r.x;
-            sum[g * 32 + i + 1] = r.y;
+          for (int i = 0; i < 32 && g + i < kMine; i += 2) {
+            const float by = S::kAligned || g + i / 16 * 16 < border ? scale : scale_beyond;
+            const float2 r = fma2(make_float2(by, by),
+                                  make_float2(__uint_as_float(d[g / 32 & 1][i]), __uint_as_float(d[g / 32 & 1][i + 1])),
+                                  make_float2(sum[g + i], sum[g + i + 1]));
+            sum[g + i] = r.x;
+            sum[g + i + 1] = r.y;
           }
         }
       }
       if (!healthy) break;
-      // The warp's 32 rows x 128 outputs leave through its own 8 KB (swizzled as the copy reads them), so that the next
+      // The warp's 32 rows leave through its own part of shared memory (swizzled as the copy reads them), so that the next
       // tile's additions start at once: all SMs end a tile together, and plain stores held them up for 3000 cycles.
-      int row_tile, col_tile;
-      tile_at(tile, row_tile, col_tile);
-      const int x = col_tile * kCols + half * kHalf, y = (row_tile * 2 + rank) * kRows + quarter * 32;
       if (lane == 0) store_wait_read<0>();
       __syncwarp();
 #pragma unroll
-      for (int piece = 0; piece < 16; ++piece) {
+      for (int piece = 0; piece < kMine / 8; ++piece) {
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = sum[piece * 8 + e];
-        st_vec(store + piece / 8 * (32 * 128) + lane * 128 + ((piece % 8 ^ (lane & 7)) << 4), pack8(v));
+        // (the swizzle exchanges 16-byte pieces by bits 7 and up of the address: by the row, or by fours of rows)
+        st_vec(store + piece / kPieces * kBoxBytes + lane * (S::kBox * 2) + ((piece % kPieces ^ (lane / (8 / kPieces) & (kPieces - 1))) << 4),
+               pack8(v));
       }
       fence_async_proxy();
       __syncwarp();
       if (lane == 0 && y < tokens) {
-        if (x < out_features) store_box(&map_out, x, y, shared_address(store));
-        if (x + 64 < out_features) store_box(&map_out, x + 64, y, shared_address(store) + 32 * 128);
+#pragma unroll
+        for (int i = 0; i < kMine / S::kBox; ++i)
+          if (x + i * S::kBox < out_features) store_box(&map_out, x + i * S::kBox, y, shared_address(store) + i * kBoxBytes);
         store_commit();
       }
     }
@@ -554,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   cluster_arrive();
   cluster_wait();  // no CTA's memory is in use by another any more
   if (warp == 2)
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kBuffers * kHalf) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   __syncwarp();
   cluster_arrive();
   cluster_wait();
@@ -819,17 +873,20 @@ EncodeTiled encoder() {
   return fn;
 }
 
-// [rows, cols] in boxes of box_rows rows of 128 bytes, swizzled; past the edges it reads as zero.
-bool encode_map(CUtensorMap* map, CUtensorMapDataType type, int element, const void* p, size_t rows, size_t cols, int box_rows) {
+// [rows, cols] in boxes of box_cols x box_rows, whose rows of 32 or 128 bytes are swizzled; past the edges it reads as zero
+// and is not written.
+bool encode_map(CUtensorMap* map, CUtensorMapDataType type, int element, const void* p, size_t rows, size_t cols, int box_cols,
+                int box_rows) {
   const EncodeTiled encode = encoder();
   if (encode == nullptr) return false;
   const cuuint64_t sizes[2] = {cols, rows}, strides[1] = {cols * element};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / element), static_cast<cuuint32_t>(box_rows)}, steps[2] = {1, 1};
-  return encode(map, type, 2, const_cast<void*>(p), sizes, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)}, steps[2] = {1, 1};
+  const CUtensorMapSwizzle swizzle = box_cols * element == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_32B;
+  return encode(map, type, 2, const_cast<void*>(p), sizes, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 bool encode_codes(CUtensorMap* map, const uint8_t* codes, size_t rows, size_t cols, int box_rows) {
-  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, rows, cols, box_rows);
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, rows, cols, kBlockK, box_rows);
 }
 
 // Opts a kernel in to its shared memory, once per device; `registers` (when not 0) is what the kernel's register split
@@ -926,19 +983,20 @@ int launch_clusters(const Problem& p, int size, int clusters, int threads, int s
   return host::launch_status();
 }
 
+template <int COLS>
 int launch_pair(const Problem& p) {
-  constexpr auto kernel = pair::block_gemm_pair_kernel;
-  const int status = prepare_kernel<kernel>(pair::kShared, pair::kLaunchRegisters);
+  using S = pair::Shape<COLS>;
+  constexpr auto kernel = pair::block_gemm_pair_kernel<COLS>;
+  const int status = prepare_kernel<kernel>(S::kShared, pair::kLaunchRegisters);
   if (status != host::kOk) return status;
   CUtensorMap a, w, o;
   if (!encode_codes(&a, p.activations, p.tokens, p.in_features, pair::kRows) ||
-      !encode_codes(&w, p.weights, p.out_features, p.in_features, pair::kHalf / 2) ||
-      !encode_map(&o, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.out, p.tokens, p.out_features, 32))
+      !encode_codes(&w, p.weights, p.out_features, p.in_features, S::kWide / 2) ||
+      !encode_map(&o, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.out, p.tokens, p.out_features, S::kBox, 32))
     return host::kNotSupported;
-  const int row_tiles = (p.tokens + 2 * pair::kRows - 1) / (2 * pair::kRows);
-  const int col_tiles = (p.out_features + pair::kCols - 1) / pair::kCols;
-  const int tiles = row_tiles * col_tiles, resident = resident_clusters<kernel, pair::kThreads>(2, pair::kShared);
-  return launch_clusters<kernel>(p, 2, tiles < resident ? tiles : resident, pair::kThreads, pair::kShared, a, w, o,
+  const int row_tiles = (p.tokens + 2 * pair::kRows - 1) / (2 * pair::kRows), col_tiles = (p.out_features + COLS - 1) / COLS;
+  const int tiles = row_tiles * col_tiles, resident = resident_clusters<kernel, pair::kThreads>(2, S::kShared);
+  return launch_clusters<kernel>(p, 2, tiles < resident ? tiles : resident, pair::kThreads, S::kShared, a, w, o,
                                  p.activation_scales, p.weight_scales, p.tokens, p.out_features, p.blocks, row_tiles, col_tiles);
 }
 
@@ -980,24 +1038,28 @@ int launch_strip(const Problem& p) {
 }
 
 // More than 64 tokens: the kernel with the least time by what each was measured to take, in hundredths of a microsecond:
-// a fixed part, then for every round of tiles on the busiest CTA so much per block of K -- panels 3 + 0.28 us
-// (128 x 5120 x 17408: 40.6 us, pairs 54.6, strips 29.2), pairs 4.5 + 0.40 us (2048 x 10240 x 5120: 89 us, panels 118), strips
-// of 128 tokens 3.6 + 0.48 us and 3.5 us for the sums of a tile (128 x 5120 x 5120: 13.9 us, panels 14.4, pairs 20.0).
+// a fixed part, then for every round of tiles on the busiest CTA so much per block of K -- panels 3 + 0.30 us
+// (200 x 5120 x 17408: 42 us, pairs of 256 outputs 50, of 160 46), pairs of 256
+// outputs 4.5 + 0.42 us (2048 x 10240 x 5120: 85 to 93 us, of 160 outputs 108, panels 122; 1337 x 5120 x 6144: 42, 51, 47), of
+// 160 outputs 4.5 + 0.35 us (512 x 10240 x 5120: 30.2 us, of 256 outputs 33.5, panels 39), strips of 128 tokens 3.6 + 0.48 us and
+// 3.5 us for the sums of a tile (128 x 5120 x 17408: 27.7 us, panels 38.4; 128 x 10240 x 5120: 24.1 us, panels 15.7).
 int launch_many(const Problem& p) {
   const long long sms = host::current_device_sm_count(), pairs = sms / 2 > 0 ? sms / 2 : 1;
   auto tiles = [&](long long rows, long long cols) {
     return (p.tokens + rows - 1) / rows * ((p.out_features + cols - 1) / cols);
   };
-  const long long panel_time = 300 + (tiles(panel::kRows, panel::kCols) + sms - 1) / sms * p.blocks * 28;
-  const long long pair_time = 450 + (tiles(2 * pair::kRows, pair::kCols) + pairs - 1) / pairs * p.blocks * 40;
+  const long long panel_time = 300 + (tiles(panel::kRows, panel::kCols) + sms - 1) / sms * p.blocks * 30;
+  const long long wide_time = 450 + (tiles(2 * pair::kRows, 256) + pairs - 1) / pairs * p.blocks * 42;
+  const long long narrow_time = 450 + (tiles(2 * pair::kRows, 160) + pairs - 1) / pairs * p.blocks * 35;
   if (p.tokens <= 128) {
     const int status = prepare_kernel<strip::block_gemm_strip_kernel<128>>(strip::Shape<128>::kShared, 0);
     if (status != host::kOk) return status;
     const StripPlan plan = plan_strip<128>(p);
     const long long strip_time = 360 + plan.rounds * (plan.blocks * 48 + 350);
-    if (strip_time < panel_time && strip_time < pair_time) return launch_strip<128>(p);
+    if (strip_time < panel_time && strip_time < wide_time && strip_time < narrow_time) return launch_strip<128>(p);
   }
-  return panel_time <= pair_time ? launch_panel(p) : launch_pair(p);
+  if (panel_time <= wide_time && panel_time <= narrow_time) return launch_panel(p);
+  return wide_time <= narrow_time ? launch_pair<256>(p) : launch_pair<160>(p);
 }
 
 }  // namespace

@@ -185,7 +185,8 @@ def test_silu_mul_non_finite(g):
 SHAPES = [(1, 8, 16), (1, 128, 128), (1, 5120, 5120), (2, 256, 1024), (3, 136, 2064), (16, 264, 144), (17, 128, 272), (31, 5120, 640),
           (33, 1000, 400), (48, 640, 17408), (64, 1024, 5120), (65, 384, 1296), (100, 24, 2048), (127, 520, 640), (128, 5120, 5120),
           (129, 256, 384), (255, 776, 1040), (256, 2048, 512), (300, 640, 6144), (512, 1288, 5120), (513, 136, 2064), (1000, 4104, 528),
-          (2049, 1032, 656), (9000, 1032, 272), (2049, 2040, 2064), (5000, 2600, 400), (4097, 4104, 656)]
+          (2049, 1032, 656), (9000, 1032, 272), (2049, 2040, 2064), (5000, 2600, 400), (4097, 4104, 656), (256, 10232, 912),
+          (500, 10072, 1040), (8193, 1000, 1168), (2000, 2600, 1296)]
 
 
 def run_gemm(g, a, sa, w, sw, stream=None):
@@ -209,7 +210,7 @@ def test_gemm(g, tokens, n, k):
 
 
 @pytest.mark.parametrize("tokens,n,k", [(1, 136, 272), (16, 256, 1040), (40, 264, 640), (100, 136, 2064), (130, 392, 528), (600, 520, 400),
-                                        (2049, 2040, 2064)])
+                                        (2049, 2040, 2064), (2000, 2600, 1296)])
 def test_gemm_keeps_non_finite_values_to_their_rows_and_columns(g, tokens, n, k):
     """A NaN code, an infinite scale and scales of zero touch the outputs they belong to and no others."""
     rng = np.random.default_rng([tokens, n, k, 29])
@@ -239,7 +240,7 @@ def test_gemm_keeps_non_finite_values_to_their_rows_and_columns(g, tokens, n, k)
 
 
 @pytest.mark.parametrize("tokens,n,k", [(1, 520, 5136), (5, 520, 5136), (16, 520, 5136), (40, 520, 5136), (100, 520, 5136), (129, 520, 5136),
-                                        (700, 520, 5136), (2049, 2040, 2064)])
+                                        (700, 520, 5136), (2049, 2040, 2064), (2000, 2600, 1296)])
 def test_gemm_repeats_bit_for_bit(g, tokens, n, k):
     """Sums are joined in one order, whatever the launch: equal inputs give equal bytes."""
     rng = np.random.default_rng([tokens, 31])
@@ -300,7 +301,7 @@ import importlib, sys
 import torch
 capi = importlib.import_module("qwen3x-orin_b200").capi
 capi.load()
-for tokens, n, k in ((1, 520, 1040), (100, 136, 2064), (200, 264, 400), (2049, 2040, 2064)):
+for tokens, n, k in ((1, 520, 1040), (100, 136, 2064), (200, 264, 400), (2049, 2040, 2064), (500, 10072, 1040)):
     blocks = (k + 127) // 128
     w, a = torch.full((n, k), 0x38, dtype=torch.uint8, device="cuda"), torch.full((tokens, k), 0x38, dtype=torch.uint8, device="cuda")
     sw, sa = torch.ones((n + 127) // 128, blocks, device="cuda"), torch.ones(blocks, tokens, device="cuda")

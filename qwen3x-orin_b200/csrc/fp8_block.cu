@@ -12,7 +12,8 @@
 //
 // Every kernel is a stream that reads its operands once.  A lane owns eight neighbouring columns (one 128-bit load per
 // operand, one 64-bit store of codes), sixteen lanes own a block, so a block's amax takes four shuffles and nothing leaves
-// registers between the arithmetic and the codes.
+// registers between the arithmetic and the codes.  Many rows are bound by HBM and, in long runs, by the power that the
+// instructions take beside it (SwiGLU of 8192 x 17408: 120 us at first, 140 after two seconds, at 1.65 GHz).
 #include <type_traits>
 
 #include "device_utils.cuh"
@@ -47,17 +48,24 @@ __device__ __forceinline__ float block_amax(float t) {
   for (int o = kBlockLanes / 2; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(kFullMask, t, o));
   return t;
 }
+// amax / 448 correctly rounded, from the rounded reciprocal, the remainder (exact: q * 448 has 27 bits) and one correction
+// (P. Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, 1990).  The quotient is A 2^s / 7
+// steps for an integer A, so at least 1/14 step away from every midpoint, and the corrected value is 2^-25 step off: it
+// rounds the same way.  (Below 2^-126 the floor decides, and nothing there comes out above it.)  Every lane does this, and
+// the streams are held back by the power that their instructions take: 8192 x 6144 28.7 -> 27.6 us against a division.
 __device__ __forceinline__ float scale_of_amax(float amax) {
-  return amax == 0.0f ? 1.0f : fmaxf(__fdiv_rn(amax, kTopE4m3), kSmallestScale);
+  constexpr float kReciprocal = 1.0f / kTopE4m3;
+  const float q = __fmul_rn(amax, kReciprocal), rest = __fmaf_rn(-q, kTopE4m3, amax);
+  return amax == 0.0f ? 1.0f : fmaxf(__fmaf_rn(rest, kReciprocal, q), kSmallestScale);
 }
 // Eight codes, column i in byte i.
 __device__ __forceinline__ uint2 encode8(const float (&y)[8], float inverse) {
   uint16_t pair[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
-        : "=h"(pair[i])
-        : "f"(__fmul_rn(y[2 * i + 1], inverse)), "f"(__fmul_rn(y[2 * i], inverse)));
+  for (int i = 0; i < 4; ++i) {  // two products per instruction, each rounded like __fmul_rn
+    const float2 q = mul2(make_float2(y[2 * i], y[2 * i + 1]), make_float2(inverse, inverse));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(pair[i]) : "f"(q.y), "f"(q.x));
+  }
   return make_uint2(pair[0] | (static_cast<uint32_t>(pair[1]) << 16), pair[2] | (static_cast<uint32_t>(pair[3]) << 16));
 }
 
@@ -215,9 +223,9 @@ void launch_quantize_deep(const uint16_t* a, const uint16_t* b, size_t row_strid
                       host::latency_bound_launch(ctas * splits), a, b, row_stride, rows, row_vectors, codes, scales);
 }
 
-// Three vectors in flight per thread once the rows alone fill the GPU (8192 x 6144: 26.9 us; one 30.3, two 29.0, four 29.1;
-// SwiGLU of 8192 x 17408: 122.5 us; 125.9, 128.9, 134.4), one while they do not (333 x 6144: 2.9 us, as with three; SwiGLU of
-// 1 x 17408 1.43 us against 1.52).
+// Three vectors in flight per thread once the rows alone fill the GPU (8192 x 6144: 26.0 us, 0.90 of a copy's rate; with scales
+// by division three took 26.9, one 30.3, two 29.0, four 29.1; SwiGLU of 8192 x 17408: 120.3 us, 0.91; 122.5, 125.9, 128.9,
+// 134.4), one while they do not (333 x 6144: 2.7 us, as with three; SwiGLU of 1 x 17408 1.4 us against 1.5).
 template <class Source, int kPerRow>
 void launch_quantize_per_row(const uint16_t* a, const uint16_t* b, size_t row_stride, size_t rows, int row_vectors, uint8_t* codes,
                              float* scales, cudaStream_t s) {
@@ -318,8 +326,9 @@ extern "C" int q3x_b200_residual_add_rms_norm_fp8_block(const uint16_t* left, co
     launch_residual_norm<decltype(depth)::value>(tokens, s, left, right, weight, row_vectors, inv_width, eps, residual_out,
                                                  normalized_out, coherent, codes, scales);
   };
-  // One vector per thread while the call is bound by latency (1 x 5120: 1.9 us, with three 2.4), three when it streams (8192 x
-  // 5120: 49.0 us; one 57.6, two 50.3, four 51.3), eight for rows beyond that.
+  // One vector per thread while the call is bound by latency (1 x 5120: 1.8 us, with three 2.4), three when it streams (8192 x
+  // 5120: 48.3 us, 0.93 of a copy's rate; with scales by division three took 49.0, one 57.6, two 50.3, four 51.3), eight for
+  // rows beyond that.
   if (row_vectors <= 64 || (row_vectors <= 1024 && latency_bound_launch(tokens))) launch(std::integral_constant<int, 1>{});
   else if (row_vectors <= 3 * kMostThreads) launch(std::integral_constant<int, 3>{});
   else launch(std::integral_constant<int, 8>{});

@@ -108,3 +108,16 @@ def test_gemm_refusals(capi):
     assert call(w=A + 8) == UNSUPPORTED and call(x=A + 2 * STEP + 8) == UNSUPPORTED and call(out=A + 4 * STEP + 8) == UNSUPPORTED
     assert call(sw=A + STEP + 2) == UNSUPPORTED and call(sx=A + 3 * STEP + 1) == UNSUPPORTED
     assert call(t=0, w=None) == OK and call(n=0, w=None) == OK
+
+
+def test_corrected_quotient_is_the_rounded_one():
+    """amax / 448 as the kernels form it -- a product with the rounded reciprocal and one correction by the exact
+    remainder -- for every mantissa of one binade (the others are its multiples by powers of two)."""
+    a = np.arange(1 << 23, 1 << 24, dtype=np.int64).astype(np.float32)
+    reciprocal = np.float32(1) / np.float32(448)
+    q = a * reciprocal
+    rest = a.astype(np.float64) - q.astype(np.float64) * 448.0  # 27 bits: exact
+    assert np.all(rest.astype(np.float32).astype(np.float64) == rest)
+    # (the sum has to be rounded once; the quotient is at least 1/14 step away from a midpoint, 64 bits of it decide)
+    corrected = (q.astype(np.longdouble) + rest.astype(np.longdouble) * np.longdouble(reciprocal)).astype(np.float32)
+    assert np.array_equal(corrected, a / np.float32(448))

@@ -78,6 +78,20 @@ def test_quantize_is_bit_exact(g, rows, cols):
     assert codes.guards_intact() and scales.guards_intact()
 
 
+def test_quantize_scales_of_every_bf16_amax(g):
+    """One block per positive finite bf16 value, subnormals included: its scale is fl(amax / 448), its codes are exact."""
+    amax = np.arange(1, 0x7F80, dtype=np.uint16)
+    x = np.zeros((amax.size, f8.BLOCK), dtype=np.uint16)
+    x[:, 77] = amax | 0x8000
+    x[:, 5] = np.maximum(amax, 0x100) - 0x80  # half of it
+    codes, scales = g.empty_like_dev(x.shape, dtype=np.uint8), g.empty_like_dev((1, amax.size), dtype=np.float32)
+    g.capi.check("q3x_b200_fp8_block_quantize", g.Dev(x), amax.size, f8.BLOCK, codes, scales, None)
+    g.sync()
+    want, want_scales = f8.quantize(bf16_values(x))
+    assert np.array_equal(scales.get(), want_scales)
+    assert np.array_equal(f8.decode(codes.get()), want)
+
+
 # ---------------------------------------------------------------------------------------------------- residual + norm
 
 

@@ -219,13 +219,14 @@ void launch_quantize_deep(const uint16_t* a, const uint16_t* b, size_t row_strid
   const size_t resident = host::resident_grid(kernel, kThreads);
   size_t splits = ctas >= resident ? 1 : (resident + ctas - 1) / ctas;
   if (splits > chunks) splits = chunks;
-  host::launch_kernel(kernel, dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(splits)), dim3(kThreads), 0, s,
-                      host::latency_bound_launch(ctas * splits), a, b, row_stride, rows, row_vectors, codes, scales);
+  // (overlapping with the kernel before takes half a microsecond off at every size: 333 x 6144 2.75 -> 2.2 us)
+  host::launch_kernel(kernel, dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(splits)), dim3(kThreads), 0, s, true, a, b,
+                      row_stride, rows, row_vectors, codes, scales);
 }
 
-// Three vectors in flight per thread once the rows alone fill the GPU (8192 x 6144: 26.0 us, 0.90 of a copy's rate; with scales
-// by division three took 26.9, one 30.3, two 29.0, four 29.1; SwiGLU of 8192 x 17408: 120.3 us, 0.91; 122.5, 125.9, 128.9,
-// 134.4), one while they do not (333 x 6144: 2.7 us, as with three; SwiGLU of 1 x 17408 1.4 us against 1.5).
+// Three vectors in flight per thread once the rows alone fill the GPU (8192 x 6144: 25.5 us, 0.91 of a copy's rate; with scales
+// by division three took 26.9, one 30.3, two 29.0, four 29.1; SwiGLU of 8192 x 17408: 118.6 us, 0.92; 122.5, 125.9, 128.9,
+// 134.4), one while they do not (333 x 6144: 2.2 us; SwiGLU of 1 x 17408 1.4 us against 1.5).
 template <class Source, int kPerRow>
 void launch_quantize_per_row(const uint16_t* a, const uint16_t* b, size_t row_stride, size_t rows, int row_vectors, uint8_t* codes,
                              float* scales, cudaStream_t s) {
@@ -254,8 +255,12 @@ void launch_residual_norm(size_t rows, cudaStream_t s, const uint16_t* left, con
                           int row_vectors, float inv_width, float eps, uint16_t* residual_out, uint16_t* normalized_out,
                           bool coherent, uint8_t* codes, float* scales) {
   const int threads = ((row_vectors + kDepth - 1) / kDepth + 31) / 32 * 32;
-  host::launch_kernel(residual_norm_fp8_kernel<kDepth>, dim3(static_cast<unsigned>(rows)), dim3(threads), 0, s,
-                      host::latency_bound_launch(rows), left, right, weight, rows, row_vectors, inv_width, eps, residual_out,
+  // Overlapping with the kernel before takes half a microsecond off (777 x 5120: 7.7 -> 7.2 us), but not where all rows are
+  // resident with room to spare: they come to lie unevenly, where the kernel before left room (333 x 5120: 4.5 -> 5.0 us).
+  // Half of an SM's 2048 threads separates the two.
+  const bool overlap =
+      host::latency_bound_launch(rows) || rows * threads >= static_cast<size_t>(host::current_device_sm_count()) * 1024;
+  host::launch_kernel(residual_norm_fp8_kernel<kDepth>, dim3(static_cast<unsigned>(rows)), dim3(threads), 0, s, overlap, left, right, weight, rows, row_vectors, inv_width, eps, residual_out,
                       normalized_out, coherent, codes, scales);
 }
 
@@ -327,7 +332,7 @@ extern "C" int q3x_b200_residual_add_rms_norm_fp8_block(const uint16_t* left, co
                                                  normalized_out, coherent, codes, scales);
   };
   // One vector per thread while the call is bound by latency (1 x 5120: 1.8 us, with three 2.4), three when it streams (8192 x
-  // 5120: 48.3 us, 0.93 of a copy's rate; with scales by division three took 49.0, one 57.6, two 50.3, four 51.3), eight for
+  // 5120: 47.8 us, 0.94 of a copy's rate; with scales by division three took 49.0, one 57.6, two 50.3, four 51.3), eight for
   // rows beyond that.
   if (row_vectors <= 64 || (row_vectors <= 1024 && latency_bound_launch(tokens))) launch(std::integral_constant<int, 1>{});
   else if (row_vectors <= 3 * kMostThreads) launch(std::integral_constant<int, 3>{});

@@ -327,7 +327,7 @@ constexpr int kRows = 128;                  // tokens of a CTA
 constexpr int kThreads = 384;               // warp 0 fetches codes, 2 scales, 1 and 3 issue (leader), 4 to 11 add up
 constexpr int kAdders = 8;                  // warps: 4 lane quarters x 2 halves of the outputs
 constexpr int kLaunchRegisters = 168;       // 65536 / 384, rounded down to 8
-constexpr int kBand = 8;                    // token tiles walked together
+constexpr size_t kBandBytes = 36u << 20;    // of activations, see band_tiles_of
 constexpr int kMostShared = 232448;         // shared memory of one CTA
 
 template <int COLS>  // outputs of a tile
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     block_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                            const __grid_constant__ CUtensorMap map_out, const float* __restrict__ sa,
                            const float* __restrict__ sw, int tokens, int out_features, int blocks, int row_tiles,
-                           int col_tiles) {
+                           int col_tiles, int band_tiles) {
   using S = Shape<COLS>;
   constexpr int kStages = S::kStages, kBuffers = S::kBuffers, kSlots = S::kSlots, kProducts = S::kProducts, kWide = S::kWide;
   extern __shared__ __align__(1024) uint8_t shared[];
@@ -412,11 +412,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   release_next_kernel();
   wait_for_prior_kernels();
 
-  // tile -> (token tile, output tile): bands of kBand token tiles, output tiles one after the other within a band, so that
-  // the tiles in flight share their operands in L2
+  // tile -> (token tile, output tile): bands of band_tiles token tiles, output tiles one after the other within a band, so
+  // that the tiles in flight share their operands in L2
   auto tile_at = [&](int tile, int& row_tile, int& col_tile) {
-    const int band = tile / (kBand * col_tiles), first = band * kBand;
-    const int height = min(kBand, row_tiles - first), rest = tile - first * col_tiles;
+    const int band = tile / (band_tiles * col_tiles), first = band * band_tiles;
+    const int height = min(band_tiles, row_tiles - first), rest = tile - first * col_tiles;
     col_tile = rest / height;
     row_tile = first + rest % height;
   };
@@ -983,6 +983,15 @@ int launch_clusters(const Problem& p, int size, int clusters, int threads, int s
   return host::launch_status();
 }
 
+// Token tiles that are walked together: as many as have their activations, which every output tile reads again, in L2 beside
+// the weights that pass through; the weights are read from memory once per band.  8192 x 34816 x 5120 in a long run: bands of
+// 8 tiles 1340 us, 16 1309, 32 1316; 8192 x 5120 x 17408, whose tiles are 3.4 times as long: 4 tiles 692 us, 8 677, 16 696.
+int band_tiles_of(const Problem& p, int row_tiles) {
+  const size_t tile_bytes = 2 * static_cast<size_t>(pair::kRows) * p.in_features;
+  const int most = static_cast<int>(pair::kBandBytes / tile_bytes), bands = most < 1 ? row_tiles : (row_tiles + most - 1) / most;
+  return (row_tiles + bands - 1) / bands;
+}
+
 template <int COLS>
 int launch_pair(const Problem& p) {
   using S = pair::Shape<COLS>;
@@ -997,7 +1006,8 @@ int launch_pair(const Problem& p) {
   const int row_tiles = (p.tokens + 2 * pair::kRows - 1) / (2 * pair::kRows), col_tiles = (p.out_features + COLS - 1) / COLS;
   const int tiles = row_tiles * col_tiles, resident = resident_clusters<kernel, pair::kThreads>(2, S::kShared);
   return launch_clusters<kernel>(p, 2, tiles < resident ? tiles : resident, pair::kThreads, S::kShared, a, w, o,
-                                 p.activation_scales, p.weight_scales, p.tokens, p.out_features, p.blocks, row_tiles, col_tiles);
+                                 p.activation_scales, p.weight_scales, p.tokens, p.out_features, p.blocks, row_tiles, col_tiles,
+                                 band_tiles_of(p, row_tiles));
 }
 
 // How a strip's tiles are shared out: the number of CTAs per tile with the fewest blocks on the busiest one, a tile's end

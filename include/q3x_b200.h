@@ -547,7 +547,7 @@ int q3x_b200_silu_mul_fp8_block(const uint16_t* gate, const uint16_t* up, size_t
 
 /* The projection of those operands, for any number of tokens from one: out[t, n] (bf16, [tokens, out_features]) =
  * sum over blocks b of activation_scales[b, t] * weight_scales[n / 128, b] * (sum over k in b of a[t, k] * w[n, k]),
- * sums in FP32, one rounding.  in_features must be a multiple of 16, out_features of 8 (cudaErrorInvalidValue).
+ * sums in FP32, one rounding.  in_features must be a positive multiple of 16, out_features of 8 (cudaErrorInvalidValue).
  * No workspace.  Every wait on the tensor cores is bounded; q3x_b200_fp8_block_gemm_error synchronises and returns the
  * current device's sticky error word (0 = no wait ever ran out, else the output of some call is not valid; -1 = the
  * word could not be read). */

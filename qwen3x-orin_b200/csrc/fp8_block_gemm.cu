@@ -882,8 +882,15 @@ bool encode_map(CUtensorMap* map, CUtensorMapDataType type, int element, const v
   const cuuint64_t sizes[2] = {cols, rows}, strides[1] = {cols * element};
   const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)}, steps[2] = {1, 1};
   const CUtensorMapSwizzle swizzle = box_cols * element == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_32B;
-  return encode(map, type, 2, const_cast<void*>(p), sizes, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  auto attempt = [&] {
+    return encode(map, type, 2, const_cast<void*>(p), sizes, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (attempt()) return true;
+  // A host thread whose first CUDA call this is has no context yet, which this one (of the driver's) wants and does not
+  // make; selecting the thread's own device does, under stream capture too.
+  int device = 0;
+  return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess && attempt();
 }
 bool encode_codes(CUtensorMap* map, const uint8_t* codes, size_t rows, size_t cols, int box_rows) {
   return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, rows, cols, kBlockK, box_rows);

@@ -5,6 +5,7 @@ import importlib
 import os
 import subprocess
 import sys
+import threading
 
 import numpy as np
 import pytest
@@ -297,6 +298,76 @@ def test_gemm_on_streams_and_in_graphs(g, tokens):
     graph.replay()
     g.sync()
     assert np.array_equal(outs[0].get(), want[1]) and np.array_equal(outs[1].get(), want[1])
+
+
+def test_calls_from_two_threads_and_graphs_of_all_kernels_at_once(g):
+    """Two threads enqueue products of every kernel on streams of their own; then two captured graphs of the same
+    products are replayed at once, again and again.  Nothing is shared between them but their inputs."""
+    rng = np.random.default_rng(47)
+    shapes = [(1, 2056, 2576), (30, 1032, 1296), (60, 520, 2064), (100, 136, 2064), (200, 1032, 1296), (500, 10072, 1040), (2049, 2040, 2064)]
+    work = []
+    for shape in shapes:
+        a, sa, w, sw = f8.operands(rng, *shape)
+        work.append((shape, [g.Dev(w), g.Dev(sw), g.Dev(a), g.Dev(sa)], run_gemm(g, a, sa, w, sw)))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[g.empty_like_dev(want.shape) for _, _, want in work] for _ in streams]
+    g.sync()
+
+    def enqueue(outs, stream, order):
+        for i in order:
+            (tokens, n, k), held, _ = work[i]
+            g.capi.check("q3x_b200_fp8_block_gemm_bf16", *held, tokens, n, k, outs[i], stream)
+
+    def verify():
+        g.sync()
+        for mine in outs:
+            for out, (shape, _, want) in zip(mine, work):
+                assert np.array_equal(out.get(), want), shape
+                assert out.guards_intact()
+                out.t.zero_()
+        assert g.capi.lib().q3x_b200_fp8_block_gemm_error() == 0
+
+    orders = [list(range(len(work))), list(reversed(range(len(work))))]
+    threads = [threading.Thread(target=lambda o=o, s=s, r=r: [enqueue(o, s.cuda_stream, r) for _ in range(10)])
+               for o, s, r in zip(outs, streams, orders)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    verify()
+    graphs = []
+    for o, r in zip(outs, orders):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            enqueue(o, torch.cuda.current_stream().cuda_stream, r)
+        graphs.append(graph)
+    for _ in range(10):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    verify()
+
+
+def test_gemm_captured_from_a_thread_that_made_no_call_before(g):
+    rng = np.random.default_rng(53)
+    shapes = [(3, 264, 400), (600, 520, 400), (2049, 2040, 2064)]
+    work = []
+    for shape in shapes:
+        a, sa, w, sw = f8.operands(rng, *shape)
+        work.append((shape, [g.Dev(w), g.Dev(sw), g.Dev(a), g.Dev(sa)], run_gemm(g, a, sa, w, sw), g.empty_like_dev(shape[:2])))
+    graph, failed = torch.cuda.CUDAGraph(), []
+    with torch.cuda.graph(graph):
+        stream = torch.cuda.current_stream().cuda_stream
+        for (tokens, n, k), held, _, out in work:
+            call = lambda: failed.append(g.capi.call("q3x_b200_fp8_block_gemm_bf16", *held, tokens, n, k, out, stream))
+            thread = threading.Thread(target=call)
+            thread.start()
+            thread.join()
+    assert failed == [0, 0, 0]
+    graph.replay()
+    g.sync()
+    for shape, _, want, out in work:
+        assert np.array_equal(out.get(), want), shape
 
 
 def test_gemm_reads_scales_from_any_float_address(g):

@@ -260,8 +260,9 @@ void launch_residual_norm(size_t rows, cudaStream_t s, const uint16_t* left, con
   // Half of an SM's 2048 threads separates the two.
   const bool overlap =
       host::latency_bound_launch(rows) || rows * threads >= static_cast<size_t>(host::current_device_sm_count()) * 1024;
-  host::launch_kernel(residual_norm_fp8_kernel<kDepth>, dim3(static_cast<unsigned>(rows)), dim3(threads), 0, s, overlap, left, right, weight, rows, row_vectors, inv_width, eps, residual_out,
-                      normalized_out, coherent, codes, scales);
+  host::launch_kernel(residual_norm_fp8_kernel<kDepth>, dim3(static_cast<unsigned>(rows)), dim3(threads), 0, s, overlap,
+                      left, right, weight, rows, row_vectors, inv_width, eps, residual_out, normalized_out, coherent, codes,
+                      scales);
 }
 
 constexpr size_t kWidestRow = kMostThreads * 8 * 8;  // eight vectors of eight columns per thread

@@ -95,7 +95,8 @@ namespace panel {
 // Tiles of 128 tokens x 128 outputs, one CTA each: for products with too few tiles of 256 x 256 to give every pair of SMs
 // one.  A block's product takes 256 cycles of the tensor cores, but its 32 KB come at 64 bytes per cycle at most, in 512:
 // that bounds it (4096 x 10240 x 5120: 65 bytes per cycle and SM leave L2, the tensor pipe is active for 51 % of the time), and
-// is why pairs take over as soon as they fill the GPU.  200 x 5120 x 17408: 41.7 us (pairs 46.2), 777 x 5120 x 6144: 35.4 us (38.7).
+// is why pairs take over as soon as they fill the GPU.  200 x 5120 x 17408: 41.7 us (pairs 46.2), 777 x 5120 x 6144: 35.4 us
+// (38.7).
 constexpr int kRows = 128;                  // tokens of a tile
 constexpr int kCols = 128;                  // outputs of a tile
 constexpr int kThreads = 384;               // warp 0 fetches codes, 2 scales, 1 and 3 issue, 4 to 11 add up
@@ -315,8 +316,8 @@ namespace pair {
 // weights' codes, and one tensor instruction runs on both SMs (cta_group::2).  Against two tiles of 128 x 256 every SM
 // fetches 32 KB instead of 48 KB per block of K, and an instruction of 128 columns reads 6 KB of shared memory instead
 // of 8 in its 64 cycles, which is what lets the accumulators be four of 128 columns: each half of the outputs has two, and
-// a half is read while three other products run.  8192 x 34816 x 5120: 1.01 to 1.13 ms from a cool start (2.6 to 2.9 PFLOP/s
-// of the 3.3 that twice the measured bf16 rate makes), 1.2 to 1.4 ms when the GPU holds its clocks down for power.
+// a half is read while three other products run.  8192 x 34816 x 5120: 1.01 to 1.15 ms from a cool start (2.5 to 2.9 PFLOP/s
+// of the 3.3 that twice the measured bf16 rate makes), 1.3 ms in a long run, where the GPU holds its clocks down for power.
 //
 // Tiles of 256 tokens x 160 outputs are for products whose tiles of 256 x 256 would leave many SMs idle in their last (or
 // only) round.  Their block is one product of all outputs, with three accumulators; their border between two weight blocks
@@ -587,8 +588,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = sum[piece * 8 + e];
         // (the swizzle exchanges 16-byte pieces by bits 7 and up of the address: by the row, or by fours of rows)
-        st_vec(store + piece / kPieces * kBoxBytes + lane * (S::kBox * 2) + ((piece % kPieces ^ (lane / (8 / kPieces) & (kPieces - 1))) << 4),
-               pack8(v));
+        const int place = piece % kPieces ^ (lane / (8 / kPieces) & (kPieces - 1));
+        st_vec(store + piece / kPieces * kBoxBytes + lane * (S::kBox * 2) + place * 16, pack8(v));
       }
       fence_async_proxy();
       __syncwarp();

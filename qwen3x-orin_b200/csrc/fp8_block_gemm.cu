@@ -626,6 +626,8 @@ namespace strip {
 // is the fixed part, some 3 us of launch, first fetch and joining of sums, and the SMs that clusters of this size leave idle.
 constexpr int kRows = 128;     // outputs of a tile
 constexpr int kMaxSplits = 8;  // CTAs of a cluster, one share of K each
+constexpr int kBuffers = 4;    // accumulators, one block of K after the other (with two, 32 x 34816 x 5120 takes 33.2 us, not
+                               // 32.7, and 128 x 5120 x 17408 28.1, not 26.9; one token does not mind)
 
 // Warp 0 fetches codes, 2 scales, 1 and 3 issue; the others add up: four for the four quarters of the lanes, and from 64
 // tokens on four more for the upper half of the tokens (128 tokens in one thread's registers: 57 us for 34816 x 5120,
@@ -642,10 +644,10 @@ struct Shape {
   static constexpr int kPartial = kStages * kStageBytes;          // [from][own group][output row] of four tokens' FP32 sums
   static constexpr int kScales = kPartial + (COLS / 4 + kMaxSplits) * kRows * 16;
   static constexpr int kBarriers = kScales + kSlots * kSlotFloats * 4;
-  static constexpr int kShared = 1024 + kBarriers + 256;
-  static constexpr int kColumns = 2 * COLS;                       // of tensor memory
-  static_assert(kStages + 2 <= kSlots, "a slot is free when the step a ring of stages earlier has left its stage");
-  static_assert(16 * kStages + 52 <= 256 && kShared <= 232448, "shared memory of one CTA");
+  static constexpr int kShared = 1024 + kBarriers + 320;
+  static constexpr int kColumns = kBuffers * COLS;                       // of tensor memory
+  static_assert(kStages + kBuffers <= kSlots, "a slot is free when the step a ring of stages earlier has left its stage");
+  static_assert(16 * kStages + 16 * kBuffers + 20 <= 320 && kShared <= 232448, "shared memory of one CTA");
 };
 
 // The cluster's CTAs share the blocks of K of one tile.  The sums of tokens 4 g to 4 g + 3 belong to rank g % splits:
@@ -661,9 +663,9 @@ __global__ void __launch_bounds__(Shape<COLS>::kThreads, 1)
   extern __shared__ uint8_t raw[];
   uint8_t* shared = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const uint32_t base = shared_address(shared);
-  const uint32_t full = base + S::kBarriers, empty = full + 8 * kStages, filled = empty + 8 * kStages, drained = filled + 16,
-                 ready = drained + 16, released = ready + 8;
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(shared + S::kBarriers + 16 * kStages + 48);
+  const uint32_t full = base + S::kBarriers, empty = full + 8 * kStages, filled = empty + 8 * kStages,
+                 drained = filled + 8 * kBuffers, ready = drained + 8 * kBuffers, released = ready + 8;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(shared + S::kBarriers + 16 * kStages + 16 * kBuffers + 16);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x % splits, cluster = blockIdx.x / splits, clusters = gridDim.x / splits;
   const int first = static_cast<int>(static_cast<long long>(blocks) * rank / splits);
@@ -676,7 +678,7 @@ __global__ void __launch_bounds__(Shape<COLS>::kThreads, 1)
       barrier_init(full + 8 * s, 1 + 32);  // the codes' fetcher and every lane of the scales'
       barrier_init(empty + 8 * s, 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kBuffers; ++i) {
       barrier_init(filled + 8 * i, 1);
       barrier_init(drained + 8 * i, S::kAdders);
     }
@@ -720,22 +722,22 @@ __global__ void __launch_bounds__(Shape<COLS>::kThreads, 1)
     for (int last = max(0, step - kStages); last < step; ++last)
       if (!wait_warp(full + 8 * (last % kStages), (last / kStages) & 1)) healthy = false;
   } else if (warp == 1 || warp == 3) {  // even and odd steps, as in the panel kernel
-    const int half = warp >> 1, steps = (tiles - cluster + clusters - 1) / clusters * count;
-    int step = half;
+    const int steps = (tiles - cluster + clusters - 1) / clusters * count;
+    int step = warp >> 1;
     for (; step < steps; step += 2) {
-      const int s = step % kStages;
+      const int s = step % kStages, buffer = step % kBuffers, round = step / kBuffers;
       if (!(healthy = wait_warp(full + 8 * s, (step / kStages) & 1))) break;
-      if (step >= 2 && !(healthy = wait_warp(drained + 8 * half, (step / 2 - 1) & 1))) break;
+      if (round > 0 && !(healthy = wait_warp(drained + 8 * buffer, (round - 1) & 1))) break;
       fence_after_sync();
       const uint32_t at = base + s * S::kStageBytes;
       if (elect_one()) {
-        block_product(tmem + half * COLS, at, at + kRows * kRowBytes, instruction_descriptor_e4m3(COLS));
+        block_product(tmem + buffer * COLS, at, at + kRows * kRowBytes, instruction_descriptor_e4m3(COLS));
         commit(empty + 8 * s);
-        commit(filled + 8 * half);
+        commit(filled + 8 * buffer);
       }
       __syncwarp();
     }
-    if (step >= 2 && !wait_warp(filled + 8 * half, (step / 2 - 1) & 1)) healthy = false;
+    if (step >= 2 && !wait_warp(filled + 8 * ((step - 2) % kBuffers), ((step - 2) / kBuffers) & 1)) healthy = false;
   } else if (warp == 2) {
     // (slots as in the panel kernel; a token past the end takes the last one's scale, its sums are not stored)
     int step = 0;
@@ -769,16 +771,16 @@ __global__ void __launch_bounds__(Shape<COLS>::kThreads, 1)
 #pragma unroll
       for (int i = 0; i < kMine; ++i) sum[i] = 0.0f;
       for (int b = 0; b < count; ++b, ++step) {
-        const int half = step & 1;
-        if (!(healthy = wait_warp(filled + 8 * half, (step / 2) & 1))) break;
+        const int buffer = step % kBuffers;
+        if (!(healthy = wait_warp(filled + 8 * buffer, (step / kBuffers) & 1))) break;
         fence_after_sync();
         const float* slot = scales + (step % S::kSlots) * S::kSlotFloats;
         const float2 weight = make_float2(slot[COLS], slot[COLS]);
 #pragma unroll
         for (int g = 0; g < kMine; g += kGroup) {
           uint32_t d[kGroup];
-          if constexpr (kGroup == 16) load16(lane_base + half * COLS + g, d);
-          else load32(lane_base + half * COLS + g, d);
+          if constexpr (kGroup == 16) load16(lane_base + buffer * COLS + g, d);
+          else load32(lane_base + buffer * COLS + g, d);
           float4 f[kGroup / 4];
 #pragma unroll
           for (int i = 0; i < kGroup / 4; ++i) f[i] = reinterpret_cast<const float4*>(slot + col0 + g)[i];
@@ -786,7 +788,7 @@ __global__ void __launch_bounds__(Shape<COLS>::kThreads, 1)
           if (g + kGroup == kMine) {
             fence_before_sync();
             __syncwarp();
-            if (lane == 0) barrier_arrive(drained + 8 * half);
+            if (lane == 0) barrier_arrive(drained + 8 * buffer);
           }
 #pragma unroll
           for (int i = 0; i < kGroup; i += 2) {
@@ -1060,7 +1062,7 @@ int launch_strip(const Problem& p) {
 // (200 x 5120 x 17408: 42 us, pairs of 256 outputs 50, of 160 46), pairs of 256
 // outputs 4.5 + 0.42 us (2048 x 10240 x 5120: 85 to 93 us, of 160 outputs 108, panels 122; 1337 x 5120 x 6144: 42, 51, 47), of
 // 160 outputs 4.5 + 0.35 us (512 x 10240 x 5120: 30.2 us, of 256 outputs 33.5, panels 39), strips of 128 tokens 3.6 + 0.48 us and
-// 3.5 us for the sums of a tile (128 x 5120 x 17408: 27.7 us, panels 38.4; 128 x 10240 x 5120: 24.1 us, panels 15.7).
+// 3.5 us for the sums of a tile (128 x 5120 x 17408: 26.9 us, panels 38.4; 128 x 10240 x 5120: 24.1 us, panels 15.7).
 int launch_many(const Problem& p) {
   const long long sms = host::current_device_sm_count(), pairs = sms / 2 > 0 ? sms / 2 : 1;
   auto tiles = [&](long long rows, long long cols) {

@@ -805,11 +805,14 @@ __global__ void __launch_bounds__(Shape<COLS>::kThreads, 1)
       const int row0 = tile / token_tiles * kRows, token0 = tile % token_tiles * COLS, visible = min(COLS, tokens - token0);
       const int groups = (visible + 3) / 4, per = (COLS / 4 + splits - 1) / splits;
       const int own = (groups + splits - 1 - rank) / splits;  // groups of this rank
-      if (warp == 4 && lane == 0) barrier_expect(ready, static_cast<uint32_t>(splits * own * kRows * 16));
       // (the first pushes wait until every CTA of the cluster has its barriers, the others until the last sums were read)
       if (!entered) cluster_wait();
       entered = true;
       if (done > 0 && !(healthy = wait_warp(released, (done - 1) & 1))) break;
+      // Only behind that wait: it says that this CTA's other adding warps have seen the last tile's phase of `ready`.  A rank
+      // without tokens completes a phase by this arrival alone, and a warp that two phases overtook would wait for good.
+      // (Sums that come before it drive the count of bytes below zero; the phase still lacks this arrival.)
+      if (warp == 4 && lane == 0) barrier_expect(ready, static_cast<uint32_t>(splits * own * kRows * 16));
       int owner = col0 / 4 % splits, place = rank * per + col0 / 4 / splits;
 #pragma unroll
       for (int i = 0; i < kMine; i += 4) {

@@ -265,6 +265,38 @@ def test_gemm_repeats_bit_for_bit(g, tokens, n, k):
         assert np.array_equal(run_gemm(g, a, sa, w, sw), first)
 
 
+# Strips whose clusters of two to five CTAs share K and walk two to five tiles each, with ranks that own no group of four tokens and
+# with ranks that all own one; and, in the last line, clusters of one CTA that walk two tiles.
+ROUNDS = [(1, 24576, 1024), (4, 24568, 1024), (1, 10240, 1040), (4, 10240, 1536), (8, 10240, 1536), (8, 20480, 1152), (5, 10248, 1168),
+          (16, 10240, 1536), (12, 13312, 5120), (7, 12288, 5120), (2, 34816, 912), (30, 10240, 1536), (24, 19456, 912), (50, 10240, 2064),
+          (64, 19464, 1168),
+          (1, 34816, 640), (48, 34816, 640)]
+
+
+@pytest.mark.parametrize("tokens,n,k", ROUNDS)
+def test_gemm_strips_of_several_tiles_per_cluster(g, tokens, n, k):
+    """Against the definition, and again and again: the barriers of a tile's end come round from tile to tile."""
+    rng = np.random.default_rng([tokens, n, k, 59])
+    a, sa, w, sw = f8.operands(rng, tokens, n, k)
+    held = [g.Dev(w), g.Dev(sw), g.Dev(a), g.Dev(sa)]
+    out = g.empty_like_dev((tokens, n), fill=0x7FC1)
+    g.capi.check("q3x_b200_fp8_block_gemm_bf16", *held, tokens, n, k, out, None)
+    g.sync()
+    first = out.get()
+    want, magnitude = f8.product(a, sa, w, sw)
+    over = np.abs(bf16_values(first).astype(np.float64) - want) - f8.product_tolerance(want, magnitude, k)
+    assert np.max(over) <= 0, f"{np.max(over)} past the tolerance at {np.unravel_index(np.argmax(over), over.shape)}"
+    expected, wrong = out.t.clone(), torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(200):
+        out.t.zero_()
+        g.capi.check("q3x_b200_fp8_block_gemm_bf16", *held, tokens, n, k, out, None)
+        wrong += (out.t != expected).sum()
+    g.sync()
+    assert int(wrong) == 0
+    assert out.guards_intact()
+    assert g.capi.lib().q3x_b200_fp8_block_gemm_error() == 0
+
+
 @pytest.mark.parametrize("tokens", [1, 24, 100, 300])
 def test_gemm_on_streams_and_in_graphs(g, tokens):
     """Two calls at once on two streams, and a captured pair replayed on new inputs."""

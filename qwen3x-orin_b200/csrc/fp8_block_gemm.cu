@@ -43,9 +43,16 @@ __device__ __forceinline__ void block_product(uint32_t accumulator, uint32_t a, 
 
 // The cluster: a barrier of all its threads in two parts, a rank's copy of an address, and an arrival on a rank's copy of a
 // barrier.  They do not publish memory to the cluster, which would cost a fence of a thousand cycles: they hand on barriers
-// and tensor memory, which have fences of their own, or say that values have been read.
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+// and tensor memory, which have fences of their own, or say that values have been read.  (Both instructions want the whole
+// warp at once, and are reached from branches that one lane takes.)
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
 __device__ __forceinline__ uint32_t at_rank(uint32_t address, int rank) {
   uint32_t there;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(address), "r"(rank));
@@ -610,7 +617,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   cluster_wait();  // no CTA's memory is in use by another any more
   if (warp == 2)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
-  __syncwarp();
   cluster_arrive();
   cluster_wait();
 }
@@ -854,7 +860,6 @@ __global__ void __launch_bounds__(Shape<COLS>::kThreads, 1)
   __syncthreads();
   if (warp == 2)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kColumns) : "memory");
-  __syncwarp();
   cluster_arrive();
   cluster_wait();  // no CTA leaves while another may still push into it
 }

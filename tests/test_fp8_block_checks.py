@@ -1,6 +1,8 @@
 """Refusals of the FP8 operators with a scale per block of 128 (they happen on the host, before any device work, so they
 run without a GPU), and the numpy restatement of the format against torch's own E4M3 type."""
 import importlib
+import os
+import re
 
 import numpy as np
 import pytest
@@ -121,3 +123,18 @@ def test_corrected_quotient_is_the_rounded_one():
     # (the sum has to be rounded once; the quotient is at least 1/14 step away from a midpoint, 64 bits of it decide)
     corrected = (q.astype(np.longdouble) + rest.astype(np.longdouble) * np.longdouble(reciprocal)).astype(np.float32)
     assert np.array_equal(corrected, a / np.float32(448))
+
+
+def test_aligned_cluster_barriers_follow_a_convergence_of_their_warp():
+    """barrier.cluster.*.aligned wants all lanes of a warp at the instruction together; its callers come from branches that
+    one lane takes (an arrival, a copy).  So each helper that issues one brings its warp together first, and nothing issues
+    one past the helpers."""
+    source = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "qwen3x-orin_b200", "csrc", "fp8_block_gemm.cu")
+    with open(source) as f:
+        text = f.read()
+    found = [m.start() for m in re.finditer(r"barrier\.cluster\.\w+[\w.]*\.aligned", text)]
+    helpers = [re.search(r"void cluster_%s\(\) \{(.*?)\n?\}" % what, text, re.S) for what in ("arrive", "wait")]
+    assert len(found) == 2
+    for helper, at in zip(helpers, found):
+        assert helper.start() < at < helper.end()
+        assert "__syncwarp();" in text[helper.start():at]

@@ -1130,6 +1130,10 @@ extern "C" int q3x_b200_fp8_block_gemm_bf16(const uint8_t* weights, const float*
 
 extern "C" int q3x_b200_fp8_block_gemm_error(void) {
   unsigned int word = 0;
-  if (cudaMemcpyFromSymbol(&word, g_error, sizeof(word)) != cudaSuccess) return -1;
+  // (the copy alone waits for the blocking streams only; a product on a non-blocking one may still be running)
+  if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(&word, g_error, sizeof(word)) != cudaSuccess) {
+    clear_stale_error();
+    return -1;
+  }
   return static_cast<int>(word);
 }

@@ -52,7 +52,8 @@ struct Fp8BlockProjectionWeight {
                                                            Fp8BlockActivation activation, std::size_t token_count,
                                                            std::uint16_t* output, void* cuda_stream = nullptr) noexcept;
 
-// The current device's sticky word: 0 = every wait of every product on the tensor cores ended in time (synchronises).
+// The current device's sticky word, read after waiting for all its streams: 0 = every wait of every product on the tensor
+// cores ended in time.
 [[nodiscard]] int fp8_block_projection_error() noexcept;
 
 }  // namespace q3x::quantization

@@ -380,6 +380,22 @@ def test_calls_from_two_threads_and_graphs_of_all_kernels_at_once(g):
     verify()
 
 
+def test_gemm_error_waits_for_streams_that_the_default_one_does_not(g):
+    """The word answers for every call enqueued before, on a non-blocking stream too."""
+    rng = np.random.default_rng(61)
+    a, sa, w, sw = f8.operands(rng, 3, 264, 400)
+    want = run_gemm(g, a, sa, w, sw)
+    held, out, side = [g.Dev(w), g.Dev(sw), g.Dev(a), g.Dev(sa)], g.empty_like_dev((3, 264)), torch.cuda.Stream()
+    g.sync()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)  # some 50 ms
+    g.capi.check("q3x_b200_fp8_block_gemm_bf16", *held, 3, 264, 400, out, side.cuda_stream)
+    assert not side.query()
+    assert g.capi.lib().q3x_b200_fp8_block_gemm_error() == 0
+    assert side.query()
+    assert np.array_equal(out.get(), want)
+
+
 def test_gemm_captured_from_a_thread_that_made_no_call_before(g):
     rng = np.random.default_rng(53)
     shapes = [(3, 264, 400), (600, 520, 400), (2049, 2040, 2064)]

@@ -493,8 +493,8 @@ int q3x_b200_gqa_attention_prefill_sigmoid_gate(const uint16_t* query, const uin
 /* The prefill attention exists twice: path 1 on tcgen05 (the default: 128 tokens of one head per CTA, scores and
  * output in tensor memory, the probabilities as two bf16 operands), path 0 on mma.sync.  Process-wide switch
  * (the environment variable Q3X_B200_GQA_PREFILL_PATH = "mma" starts on path 0).  Path 1 bounds every wait on the
- * tensor cores; q3x_b200_gqa_prefill_tcgen05_error synchronises and returns its sticky error word (0 = no wait ever
- * ran out, -1 = the word could not be read). */
+ * tensor cores; q3x_b200_gqa_prefill_tcgen05_error waits for all streams of the current device and returns its sticky
+ * error word (0 = no wait ever ran out, -1 = the word could not be read).  Not for use during a capture. */
 int q3x_b200_gqa_prefill_select_path(int path);
 int q3x_b200_gqa_prefill_tcgen05_error(void);
 

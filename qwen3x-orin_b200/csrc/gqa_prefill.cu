@@ -592,6 +592,10 @@ extern "C" int q3x_b200_gqa_prefill_select_path(int path) {
 
 extern "C" int q3x_b200_gqa_prefill_tcgen05_error(void) {
   unsigned int word = 0;
-  if (cudaMemcpyFromSymbol(&word, tcattn::g_error, sizeof(word)) != cudaSuccess) return -1;
+  // (the copy alone waits for the blocking streams only; a tile on a non-blocking one may still be running)
+  if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(&word, tcattn::g_error, sizeof(word)) != cudaSuccess) {
+    clear_stale_error();
+    return -1;
+  }
   return static_cast<int>(word);
 }

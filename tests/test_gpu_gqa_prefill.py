@@ -186,3 +186,19 @@ def test_prefill_attention_rejections(g):
     assert call(s=0.0) == inv
     assert call(out=fake) == inv
     assert call(t=0) == 0
+
+
+def test_prefill_error_waits_for_streams_that_the_default_one_does_not(g):
+    """The word answers for every tile enqueued before, on a non-blocking stream too."""
+    rng = np.random.default_rng(113)
+    q, kc, vc = g.Dev(fx.normal_bf16(rng, (40, 24, 256))), g.Dev(fx.normal_bf16(rng, (40, 4, 256))), g.Dev(fx.normal_bf16(rng, (40, 4, 256)))
+    out, apart, side = g.empty_like_dev((40, 24, 256)), g.empty_like_dev((40, 24, 256)), torch.cuda.Stream()
+    g.capi.check("q3x_b200_gqa_attention_prefill_sigmoid_gate", q, kc, vc, None, 0, 40, SCALE, apart, None)
+    g.sync()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)  # some 50 ms
+    g.capi.check("q3x_b200_gqa_attention_prefill_sigmoid_gate", q, kc, vc, None, 0, 40, SCALE, out, side.cuda_stream)
+    assert not side.query()
+    assert g.capi.lib().q3x_b200_gqa_prefill_tcgen05_error() == 0
+    assert side.query()
+    assert np.array_equal(out.get(), apart.get())

@@ -7,10 +7,12 @@
 #pragma once
 #include <cstdint>
 
+#include "bounded_wait.hpp"
+
 namespace q3x {
 namespace tcgen05 {
 
-constexpr uint32_t kWaitLimit = 1u << 20;  // (and 50 ms, whichever comes first)
+constexpr uint32_t kWaitLimit = 1u << 20;  // polls (and 50 ms, whichever comes first)
 
 // K-major operand ([rows][k], k contiguous) of 64-element rows; groups of eight rows 1024 bytes apart
 __device__ __forceinline__ uint64_t operand_descriptor(uint32_t shared_address) {
@@ -39,23 +41,25 @@ __device__ __forceinline__ void product(uint32_t accumulator, uint32_t a_base, u
 __device__ __forceinline__ void commit(uint32_t barrier) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(barrier) : "memory");
 }
+// Whether the phase is complete; one that is not may hold the warp, until it is or for some microseconds.
+__device__ __forceinline__ bool barrier_try(uint32_t barrier, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(done)
+               : "r"(barrier), "r"(parity)
+               : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ uint64_t wall_clock() {
+  uint64_t now;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+  return now;
+}
 // A wait on the completion barrier that is bounded in TIME (50 ms on the global timer; a product here completes in
-// microseconds): false means it ran out.
+// microseconds): false means it ran out.  (The first poll, which mostly ends it, comes before the timer is read.)
 __device__ __forceinline__ bool wait(uint32_t barrier, uint32_t parity) {
-  uint64_t start;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
-  for (uint32_t spin = 0; spin < kWaitLimit; ++spin) {
-    uint32_t done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(done)
-                 : "r"(barrier), "r"(parity)
-                 : "memory");
-    if (done) return true;
-    uint64_t now;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
-    if (now - start > 50000000ull) return false;
-  }
-  return false;
+  return barrier_try(barrier, parity) ||
+         wait_in_time([=] { return barrier_try(barrier, parity); }, [] { return wall_clock(); }, 50000000ull, kWaitLimit);
 }
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -134,28 +138,12 @@ __device__ __forceinline__ void barrier_expect(uint32_t barrier, uint32_t bytes)
 __device__ __forceinline__ void barrier_arrive(uint32_t barrier) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(barrier) : "memory");
 }
-// Whether the phase is complete; one that is not may hold the warp, until it is or for some microseconds.
-__device__ __forceinline__ bool barrier_try(uint32_t barrier, uint32_t parity) {
-  uint32_t done;
-  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-               : "=r"(done)
-               : "r"(barrier), "r"(parity)
-               : "memory");
-  return done != 0;
-}
 // The bounded wait for kernels that wait once per tile of a long loop: the timer is only read after a thousand polls
 // (it costs more than a completed wait), and the bound is 200 ms.
 __device__ __forceinline__ bool wait_bounded(uint32_t barrier, uint32_t parity) {
   for (int spin = 0; spin < 1024; ++spin)
     if (barrier_try(barrier, parity)) return true;
-  uint64_t start, now;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
-  for (uint32_t spin = 0; spin < (1u << 28); ++spin) {
-    if (barrier_try(barrier, parity)) return true;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
-    if (now - start > 200000000ull) return false;
-  }
-  return false;
+  return wait_in_time([=] { return barrier_try(barrier, parity); }, [] { return wall_clock(); }, 200000000ull, 1u << 28);
 }
 // Box of a two-dimensional tensor map at (x, y) into this CTA's shared memory; completes `bytes` on the barrier.
 __device__ __forceinline__ void load_box(uint32_t shared_address, const void* map, int x, int y, uint32_t barrier) {

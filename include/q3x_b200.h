@@ -547,7 +547,9 @@ int q3x_b200_silu_mul_fp8_block(const uint16_t* gate, const uint16_t* up, size_t
 
 /* The projection of those operands, for any number of tokens from one: out[t, n] (bf16, [tokens, out_features]) =
  * sum over blocks b of activation_scales[b, t] * weight_scales[n / 128, b] * (sum over k in b of a[t, k] * w[n, k]),
- * sums in FP32, one rounding.  in_features must be a positive multiple of 16, out_features of 8 (cudaErrorInvalidValue).
+ * sums in FP32, one rounding.  The two scales are multiplied with each other first, in FP32: where their product leaves its
+ * normal range (below 2^-126, e.g. the smallest activation scale times a weight scale below 1; 2^128 and up) it is a subnormal, 0 or
+ * infinite, whatever the sum it meets.  in_features must be a positive multiple of 16, out_features of 8 (cudaErrorInvalidValue).
  * No workspace.  Every wait on the tensor cores is bounded; q3x_b200_fp8_block_gemm_error waits for all streams of the
  * current device and returns its sticky error word (0 = no wait ever ran out, else the output of some call since the
  * process began is not valid, -1 = the word could not be read).  Nothing clears it.  Not for use during a capture. */

@@ -2,7 +2,9 @@
 //   out[t, n] = bf16( sum over blocks b of sa[b, t] * sw[n / 128, b] * (sum over k in b of a[t, k] * w[n, k]) )
 // sa [ceil(K / 128), T] as the quantisers of fp8_block.cu write it, sw [ceil(N / 128), ceil(K / 128)].  A block's products
 // are summed in FP32 by the tensor cores, multiplied by the two scales and added to the running FP32 sum; the one rounding
-// is to bf16.
+// is to bf16.  The scales are multiplied with each other first, once per token and block, so that an output costs one fused
+// multiply and add per block (the additions set the pace of some tiles, see below); the price is that a product of
+// scales outside FP32's range is lost even where the sum would have brought it back.
 //
 // Three kernels on tcgen05 (kind::f8f6f4: E4M3 x E4M3 -> FP32 in tensor memory), operands fetched by bulk tensor copies
 // into rings of 128-byte-swizzled stages, one stage per block of 128 columns of K:

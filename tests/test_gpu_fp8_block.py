@@ -254,6 +254,29 @@ def test_gemm_keeps_non_finite_values_to_their_rows_and_columns(g, tokens, n, k)
     assert np.array_equal(got[~bad], clean[~bad])
 
 
+@pytest.mark.parametrize("tokens,n,k", [(6, 264, 400), (30, 264, 400), (60, 392, 528), (128, 5120, 5120), (200, 264, 400), (500, 10072, 1040),
+                                        (2049, 2040, 2064)])
+def test_gemm_multiplies_the_scales_first(g, tokens, n, k):
+    """Scales whose product is small, subnormal, 0, large or infinite in FP32: that product is what the sum is multiplied by."""
+    rng = np.random.default_rng([tokens, n, k, 67])
+    # (codes of 1/4 to 15/8, so that no block's sum is 0 and the products stay in range wherever the factor does)
+    a, w = (rng.integers(0x28, 0x40, size=shape, dtype=np.uint8) for shape in ((tokens, k), (n, k)))
+    row = np.resize(np.exp2([-126.0, -100, 0, 90, 119, -120]).astype(np.float32) * np.float32(1.25), tokens)
+    col = np.resize(np.exp2([-30.0, -12, 20]).astype(np.float32) * np.float32(1.375), f8.blocks_of(n))
+    sa, sw = np.tile(row, (f8.blocks_of(k), 1)), np.tile(col[:, None], (1, f8.blocks_of(k)))
+    got = bf16_values(run_gemm(g, a, sa, w, sw)).astype(np.float64)
+    with np.errstate(over="ignore", under="ignore"):
+        factor = (row[:, None] * np.repeat(col, f8.BLOCK)[None, :n]).astype(np.float64)
+    assert factor.min() == 0 and np.isinf(factor.max())
+    want = factor * (f8.decode(a) @ f8.decode(w).T)
+    fine = np.isfinite(want)
+    assert np.array_equal(got[~fine], want[~fine])
+    assert np.all(got[factor == 0] == 0)
+    # (all terms are positive: their sum is their magnitude)
+    got, want = got[fine], want[fine]
+    assert np.all(np.abs(got - want) <= f8.product_tolerance(want, want, k))
+
+
 @pytest.mark.parametrize("tokens,n,k", [(1, 520, 5136), (5, 520, 5136), (16, 520, 5136), (40, 520, 5136), (100, 520, 5136), (129, 520, 5136),
                                         (700, 520, 5136), (2049, 2040, 2064), (2000, 2600, 1296)])
 def test_gemm_repeats_bit_for_bit(g, tokens, n, k):

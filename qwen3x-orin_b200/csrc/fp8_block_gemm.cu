@@ -104,8 +104,8 @@ namespace panel {
 // Tiles of 128 tokens x 128 outputs, one CTA each: for products with too few tiles of 256 x 256 to give every pair of SMs
 // one.  A block's product takes 256 cycles of the tensor cores, but its 32 KB come at 64 bytes per cycle at most, in 512:
 // that bounds it (4096 x 10240 x 5120: 65 bytes per cycle and SM leave L2, the tensor pipe is active for 51 % of the time), and
-// is why pairs take over as soon as they fill the GPU.  200 x 5120 x 17408: 41.7 us (pairs 46.2), 777 x 5120 x 6144: 35.4 us
-// (38.7).
+// is why pairs take over as soon as they fill the GPU.  200 x 5120 x 17408: 40.0 us (pairs 45.7), 777 x 5120 x 6144: 32.2 us
+// (34.9).
 constexpr int kRows = 128;                  // tokens of a tile
 constexpr int kCols = 128;                  // outputs of a tile
 constexpr int kThreads = 384;               // warp 0 fetches codes, 2 scales, 1 and 3 issue, 4 to 11 add up
@@ -325,18 +325,22 @@ namespace pair {
 // weights' codes, and one tensor instruction runs on both SMs (cta_group::2).  Against two tiles of 128 x 256 every SM
 // fetches 32 KB instead of 48 KB per block of K, and an instruction of 128 columns reads 6 KB of shared memory instead
 // of 8 in its 64 cycles, which is what lets the accumulators be four of 128 columns: each half of the outputs has two, and
-// a half is read while three other products run.  8192 x 34816 x 5120: 1.01 to 1.15 ms from a cool start (2.5 to 2.9 PFLOP/s
-// of the 3.3 that twice the measured bf16 rate makes), 1.3 ms in a long run, where the GPU holds its clocks down for power.
+// a half is read while three other products run.  8192 x 34816 x 5120: 1.12 to 1.16 ms from a cool start (2.5 to 2.6 PFLOP/s
+// of the 3.3 that twice the measured bf16 rate makes), 1.31 to 1.35 ms in a long run, where the GPU holds its clocks down for
+// power.
 //
 // Tiles of 256 tokens x 160 outputs are for products whose tiles of 256 x 256 would leave many SMs idle in their last (or
 // only) round.  Their block is one product of all outputs, with three accumulators; their border between two weight blocks
-// can lie anywhere.  256 x 10240 x 5120: 17.4 us (256 outputs 20.4, panels 25.9), 512 x 10240 x 5120: 30.2 us (33.5, 39).
+// can lie anywhere.  256 x 10240 x 5120: 17.6 us (256 outputs 20.3, panels 25.4), 512 x 10240 x 5120: 31.7 us (33.5, 36.4).
 // A block takes 0.31 us with few SMs at work; with the additions left out 0.24, with three of four products left out too the
-// same: fetching it, 26 KB per SM at 64 bytes per cycle, is the bound.  (Tiles of 96 or 128 outputs: 0.28 us.)
+// same.  So fetching it, 26 KB per SM at 64 bytes per cycle, is the floor of 0.24 us, and the adding warps, which read an
+// accumulator in three loads with a wait each before they give it back, cost the other 0.07.  (Tiles of 96 or 128 outputs:
+// 0.28 us.)
 constexpr int kRows = 128;                  // tokens of a CTA
 constexpr int kThreads = 384;               // warp 0 fetches codes, 2 scales, 1 and 3 issue (leader), 4 to 11 add up
 constexpr int kAdders = 8;                  // warps: 4 lane quarters x 2 halves of the outputs
-constexpr int kLaunchRegisters = 168;       // 65536 / 384, rounded down to 8
+constexpr int kLaunchRegisters = 168;       // 65536 / 384, rounded down to 8; the compiler spills a little all the same: 24 bytes
+                                            // stored and 64 loaded with 256 outputs, 20 and 64 with 160
 constexpr size_t kBandBytes = 36u << 20;    // of activations, see band_tiles_of
 constexpr int kMostShared = 232448;         // shared memory of one CTA
 
@@ -630,7 +634,7 @@ namespace strip {
 
 // Outputs are the rows of the product, so that one token costs 16 columns and not a tile of 128 rows.  All that counts is to
 // keep the weights coming: 131 to 202 KB of them are in flight per SM, and K is split until every SM has a share.  One token,
-// 34816 x 5120: 30.1 us, 5.9 TB/s (0.90 of what a copy reaches); 5120 x 17408: 17.0 us (0.80); 48 tokens: 19.4 us.  What is left
+// 34816 x 5120: 29.9 us, 6.0 TB/s (0.91 of what a copy reaches); 5120 x 17408: 17.1 us (0.80); 48 tokens: 19.2 us.  What is left
 // is the fixed part, some 3 us of launch, first fetch and joining of sums, and the SMs that clusters of this size leave idle.
 constexpr int kRows = 128;     // outputs of a tile
 constexpr int kMaxSplits = 8;  // CTAs of a cluster, one share of K each
@@ -639,7 +643,7 @@ constexpr int kBuffers = 4;    // accumulators, one block of K after the other (
 
 // Warp 0 fetches codes, 2 scales, 1 and 3 issue; the others add up: four for the four quarters of the lanes, and from 64
 // tokens on four more for the upper half of the tokens (128 tokens in one thread's registers: 57 us for 34816 x 5120,
-// bound by the additions).
+// bound by the additions; with 64 each 12 bytes are still spilled).
 template <int COLS>
 struct Shape {
   static constexpr int kAdders = COLS >= 64 ? 8 : 4;
@@ -1069,10 +1073,13 @@ int launch_strip(const Problem& p) {
 
 // More than 64 tokens: the kernel with the least time by what each was measured to take, in hundredths of a microsecond:
 // a fixed part, then for every round of tiles on the busiest CTA so much per block of K -- panels 3 + 0.30 us
-// (200 x 5120 x 17408: 42 us, pairs of 256 outputs 50, of 160 46), pairs of 256
-// outputs 4.5 + 0.42 us (2048 x 10240 x 5120: 85 to 93 us, of 160 outputs 108, panels 122; 1337 x 5120 x 6144: 42, 51, 47), of
-// 160 outputs 4.5 + 0.35 us (512 x 10240 x 5120: 30.2 us, of 256 outputs 33.5, panels 39), strips of 128 tokens 3.6 + 0.48 us and
-// 3.5 us for the sums of a tile (128 x 5120 x 17408: 26.9 us, panels 38.4; 128 x 10240 x 5120: 24.1 us, panels 15.7).
+// (200 x 5120 x 17408: 40.0 us, pairs of 256 outputs 50.2, of 160 45.6), pairs of 256
+// outputs 4.5 + 0.42 us (2048 x 10240 x 5120: 92.9 us, of 160 outputs 108.5, panels 118.5; 1337 x 5120 x 6144: 43.4, 51.9, 48.7), of
+// 160 outputs 4.5 + 0.35 us (512 x 10240 x 5120: 31.7 us, of 256 outputs 33.5, panels 36.4), strips of 128 tokens 3.6 + 0.48 us and
+// 3.5 us for the sums of a tile (128 x 5120 x 17408: 26.6 us, panels 38.3; 128 x 10240 x 5120: 23.2 us, panels 15.7).
+// The times are those of full rounds.  A round with few tiles is shorter than the model has it (200 x 5120 x 17408 on pairs of
+// 256 outputs 61.6 us against 50.2, 512 x 10240 x 5120 38.1 against 33.5) and long runs of rounds are longer (4096 x 10240 x 5120 156
+// against 174): the errors of the kernels go the same way, and at each of these sizes the least time was the chosen one's.
 int launch_many(const Problem& p) {
   const long long sms = host::current_device_sm_count(), pairs = sms / 2 > 0 ? sms / 2 : 1;
   auto tiles = [&](long long rows, long long cols) {

@@ -18,8 +18,8 @@ constexpr uint64_t kMostPerPoll = 1000000;  // nanoseconds
 // wall's: it runs on while the process is switched off the GPU, between a poll that failed and the reading of the clock as
 // well, and what is waited for stands still meanwhile.  So the time from one poll to the next counts for a millisecond at
 // most: time away counts as one poll, and a barrier that was complete, or completes soon after, is seen by those that
-// follow.  (A poll may hold its thread for some microseconds; were it longer than a millisecond, the bound would be `limit`
-// polls of a millisecond each, whatever they take.)
+// follow.  (A poll may hold its thread for some microseconds; were it longer than a millisecond, the bound would be as many
+// polls as `limit` has milliseconds.)
 template <class Poll, class Clock>
 Q3X_WAIT_FUNCTION bool wait_in_time(const Poll& poll, const Clock& clock, uint64_t limit, uint32_t most_polls) {
   uint64_t last = clock(), waited = 0;
